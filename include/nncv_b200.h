@@ -71,7 +71,7 @@ enum {
   NNCV_B200_ENOMEM = 7
 };
 
-enum { NNCV_B200_F32 = 0, NNCV_B200_F16 = 1, NNCV_B200_BF16 = 2 };
+enum { NNCV_B200_F32 = 0, NNCV_B200_F16 = 1, NNCV_B200_BF16 = 2, NNCV_B200_E4M3 = 3 /* operands of nncv_b200_matmul_e4m3 only */ };
 
 typedef struct {
   int compute_dtype; /* NNCV_B200_F32 (fp32 accuracy: three bf16 planes per operand, tcgen05; activations take 6 bytes an
@@ -347,6 +347,37 @@ int nncv_b200_concat_channels_nhwc(const void* const* inputs, const int* channel
 /* Nearest-neighbour 2x upsampling (Yolov5s.mlir:876-884: tensor.extract at floordivsi(index, 2)):
  * in [N,H,W,C] -> out [N,2H,2W,C]. */
 int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H, int W, int C, void* stream);
+
+/* ---- a linear layer in 8-bit floating point (device pointers; `stream` is a cudaStream_t; no synchronisation) ----
+ * No counterpart in the reference, whose matmuls are 16-bit and fp32.  Values are e4m3 (one byte: 4 exponent bits, 3 mantissa
+ * bits, largest 448, no infinity) with one fp32 scale for each block of 128: value = byte * scale.  A block of values y is written
+ * with scale = max(largest finite |y|, 2^-100) / 448 and y / scale rounded to nearest; an infinity or a NaN becomes NaN and
+ * leaves the rest of its block as it is.  Scales of an [M,K] matrix: [M, ceil(K/128)] (activations: one for 128 columns of a row) or
+ * [ceil(M/128), ceil(K/128)] (weights: one for 128 x 128), row-major; the last block of a row may be shorter.
+ * Rows of x, gate and up may lie further apart than K (ldx, ld: elements from row to row, 0 = K); all else is dense.  M = 0 is
+ * a call that does nothing.  Everything computes in fp32; an fp16 result beyond its range becomes +-65504.  Any K and any
+ * address of an element are allowed; K a multiple of 8 with everything on 16-byte boundaries is read 16 bytes at a time.
+ *
+ * Root-mean-square norm of x, or of h = x + residual: out = h / sqrt(mean(h^2) + eps) * weight.
+ *   x [M,K] of dtype; residual [M,K] of dtype or NULL; weight fp32 [K] or NULL (= 1); K up to 32768
+ *   sum: NULL, or [M,K] of dtype that receives h (the norm is taken of h before this rounding); may be residual, or x where ldx is K
+ *   out: [M,K] of out_dtype, which is dtype or NNCV_B200_E4M3; scale: fp32 [M, ceil(K/128)] with E4M3, else NULL
+ * out may be x (where ldx is K) or residual, if it has their type. */
+int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const void* weight, float eps, void* sum, void* out, int out_dtype,
+                      float* scale, int dtype, int M, int K, void* stream);
+/* out = activation(gate) * up, or activation(gate) where up is NULL.  gate and up [M,K] of dtype, rows ld apart: the halves of one
+ * [M,2K] tensor are gate = t, up = t + K, ld = 2K.  act: NNCV_B200_ACT_*.  out and scale as above; out may be gate or up where ld is K and the
+ * types agree. */
+int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, void* out, int out_dtype, float* scale, int dtype, int M, int K,
+                               int act, void* stream);
+/* x [M,K] of dtype to e4m3 q [M,K] with a scale for block_rows x 128 values, block_rows 1 or 128. */
+int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, float* scale, int M, int K, int block_rows, void* stream);
+/* C[M,N] = A * B^T (+ bias[N]) (+ ReLU): A [M,K] e4m3 with scales [M, ceil(K/128)], B [N,K] e4m3 (as a fully connected layer stores
+ * its weights) with scales [ceil(N/128), ceil(K/128)]; C of c_dtype F32, F16 or BF16.  K a multiple of 16, A and B on 16-byte boundaries, C on any
+ * element's.  fp32 sums; a block's sum is scaled before it is added to the others.  No scratch: calls on several streams, and captured
+ * calls, share nothing. */
+int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, const float* scale_b, void* C, int M, int N, int K, int c_dtype,
+                          const float* bias, int relu, void* stream);
 
 #ifdef __cplusplus
 }

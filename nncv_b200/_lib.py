@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_int, c_longlong, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_longlong, c_size_t, c_void_p
 
 from .memref import MemRefDescriptor1, MemRefDescriptor2, MemRefDescriptor4, MemRefIndexer
 
@@ -30,9 +30,10 @@ EXPORTS = [
     "nncv_b200_matmul", "nncv_b200_matmul_noalloc", "nncv_b200_conv_create", "nncv_b200_conv_destroy", "nncv_b200_conv_run",
     "nncv_b200_conv_run_fused", "nncv_b200_conv_set_tile", "nncv_b200_stem_pool", "nncv_b200_stem_variant",
     "nncv_b200_maxpool_nhwc", "nncv_b200_avgpool_nhwc", "nncv_b200_nchw_to_nhwc", "nncv_b200_bn_fold",
+    "nncv_b200_rmsnorm", "nncv_b200_gated_activation", "nncv_b200_quantize_e4m3", "nncv_b200_matmul_e4m3",
 ]
 
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 
 
 class ProfRec(ctypes.Structure):
@@ -121,6 +122,11 @@ def lib() -> ctypes.CDLL:
                                          c_void_p]
     L.nncv_b200_bn_fold.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p,
                                     c_void_p]
+    L.nncv_b200_rmsnorm.argtypes = [c_void_p, c_longlong, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
+                                    c_void_p]
+    L.nncv_b200_gated_activation.argtypes = [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
+    L.nncv_b200_quantize_e4m3.argtypes = [c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]
+    L.nncv_b200_matmul_e4m3.argtypes = [c_void_p] * 5 + [c_int] * 4 + [c_void_p, c_int, c_void_p]
     _lib = L
     return L
 

@@ -295,6 +295,51 @@ cudaError_t launch_se(void* x, Layout l, const float* w1, const float* b1, const
 cudaError_t launch_concat(const void* const* in, const int* channels, int n_in, void* out, DType dt, long long pixels, cudaStream_t st);
 cudaError_t launch_upsample2x(const void* in, void* out, DType dt, int N, int H, int W, int C, cudaStream_t st);
 
+// ---- a linear layer in 8 bits: e4m3 values with an fp32 scale for every block of 128 (value = q * scale) ----
+constexpr int kRmsNormMaxK = 32768;    // a row stays in the registers of one CTA
+struct RmsNormArgs {
+  const void* x = nullptr;             // [M,K], rows ldx elements apart
+  long long ldx = 0;
+  const void* residual = nullptr;      // [M,K] or null
+  const float* weight = nullptr;       // [K] or null (=1)
+  float eps = 0.0f;
+  void* sum = nullptr;                 // x + residual, or null
+  void* out = nullptr;                 // [M,K] of dtype, or e4m3
+  float* scale = nullptr;              // [M,ceil(K/128)] (e4m3)
+  DType dtype = kF16;
+  bool to_e4m3 = false;
+  int M = 0, K = 0;
+};
+cudaError_t launch_rmsnorm(const RmsNormArgs& a, cudaStream_t st);
+struct GatedArgs {
+  const void* gate = nullptr;          // [M,K], rows ld elements apart
+  const void* up = nullptr;            // the same, or null (=1)
+  long long ld = 0;
+  void* out = nullptr;                 // [M,K] of dtype, or e4m3
+  float* scale = nullptr;              // [M,ceil(K/128)] (e4m3)
+  DType dtype = kF16;
+  bool to_e4m3 = false;
+  int M = 0, K = 0, act = 0;
+  int sm_count = 0;
+};
+cudaError_t launch_gated_activation(const GatedArgs& a, cudaStream_t st);
+// One scale for each 128 x 128 block.
+cudaError_t launch_quantize_blocks(const void* x, long long ldx, DType dt, void* q, float* scale, int M, int K, cudaStream_t st);
+struct GemmE4m3Args {
+  const void* A = nullptr;             // [M,K]
+  const float* scale_a = nullptr;      // [M,ceil(K/128)]
+  const void* B = nullptr;             // [N,K]
+  const float* scale_b = nullptr;      // [ceil(N/128),ceil(K/128)]
+  void* C = nullptr;                   // [M,N] of c_dtype
+  const float* bias = nullptr;         // [N] or null
+  DType c_dtype = kF32;
+  int relu = 0;
+  int M = 0, N = 0, K = 0;
+  int sm_count = 0;
+  int* error_flag = nullptr;
+};
+cudaError_t launch_gemm_e4m3(const GemmE4m3Args& a, cudaStream_t st);
+
 // ---- activation arena planning (host only) ----------------------------------------------------
 struct ArenaTensor {
   int first = 0, last = 0;   // ops that produce it / read it last, both included

@@ -336,6 +336,18 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
       : "memory");
 }
+// The same on 8-bit floating-point operands, 32 k values (32 bytes) an instruction.
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
+      : "memory");
+}
 // A in tensor memory: row i of the tile in lane i, one k value a column.
 __device__ __forceinline__ void umma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
   asm volatile(
@@ -622,8 +634,8 @@ __device__ __forceinline__ uint64_t desc_from_halves(uint32_t lo, uint32_t hi) {
   return d;
 }
 
-// Instruction descriptor of tcgen05.mma kind::f16 / kind::tf32, fp32 accumulate, both operands
-// K-major.  ab_format: 0 = fp16, 1 = bf16, 2 = tf32.
+// Instruction descriptor of tcgen05.mma kind::f16 / kind::tf32 / kind::f8f6f4, fp32 accumulate, both operands
+// K-major.  ab_format: 0 = fp16, 1 = bf16, 2 = tf32; of kind::f8f6f4: 0 = e4m3.
 //   bits [4,6) D format (1 = f32)   [7,10) A format   [10,13) B format
 //   bit 15 / 16 A / B major (0 = K)  [17,23) N >> 3    [24,29) M >> 4
 __host__ __device__ constexpr uint32_t umma_idesc(int m, int n, int ab_format) {

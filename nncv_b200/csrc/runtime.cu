@@ -3084,4 +3084,93 @@ int nncv_b200_bn_fold(const void* gamma, const void* beta, const void* mean, con
   return ok();
 }
 
+// ---- a linear layer in 8 bits -------------------------------------------------------------
+static bool on_boundary(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+static bool of_type(const void* p, int dtype) { return on_boundary(p, dtype_size((DType)dtype)); }
+// out_dtype is dtype or E4M3, and scales go with E4M3 alone
+static int check_out(const char* what, int out_dtype, int dtype, const void* out, const float* scale) {
+  if (out_dtype != dtype && out_dtype != NNCV_B200_E4M3) return fail(NNCV_B200_EINVAL, "%s: out_dtype must be dtype or E4M3", what);
+  if ((out_dtype == NNCV_B200_E4M3) != (scale != nullptr)) return fail(NNCV_B200_EINVAL, "%s: scale goes with an E4M3 result, and only with one", what);
+  if ((out_dtype != NNCV_B200_E4M3 && !of_type(out, dtype)) || !on_boundary(scale, 4)) return fail(NNCV_B200_EINVAL, "%s: a pointer is not on its type's boundary", what);
+  return NNCV_B200_OK;
+}
+
+int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const void* weight, float eps, void* sum, void* out, int out_dtype,
+                      float* scale, int dtype, int M, int K, void* stream) {
+  std::lock_guard<std::mutex> lk(g_mutex);
+  int rc = NNCV_B200_OK;
+  if (!x || !out || M < 0 || K <= 0 || dtype < 0 || dtype > 2 || !(eps >= 0.0f)) return fail(NNCV_B200_EINVAL, "rmsnorm: bad argument");
+  if (K > kRmsNormMaxK) return fail(NNCV_B200_EINVAL, "rmsnorm: K may be at most %d", kRmsNormMaxK);
+  if (ldx == 0) ldx = K;
+  if (ldx < K) return fail(NNCV_B200_EINVAL, "rmsnorm: ldx is less than K");
+  if (!of_type(x, dtype) || !of_type(residual, dtype) || !of_type(sum, dtype) || !on_boundary(weight, 4))
+    return fail(NNCV_B200_EINVAL, "rmsnorm: a pointer is not on its type's boundary");
+  if ((rc = check_out("rmsnorm", out_dtype, dtype, out, scale))) return rc;
+  if (ldx != K && (sum == x || out == x)) return fail(NNCV_B200_EINVAL, "rmsnorm: a result may take the place of x only where ldx is K");
+  if (out == sum || (out_dtype == NNCV_B200_E4M3 && (out == x || out == residual))) return fail(NNCV_B200_EINVAL, "rmsnorm: out needs memory of its own");
+  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  RmsNormArgs a;
+  a.x = x; a.ldx = ldx; a.residual = residual; a.weight = (const float*)weight; a.eps = eps; a.sum = sum; a.out = out; a.scale = scale;
+  a.dtype = (DType)dtype; a.to_e4m3 = out_dtype == NNCV_B200_E4M3; a.M = M; a.K = K;
+  LAUNCH(launch_rmsnorm(a, (cudaStream_t)stream));
+  return ok();
+}
+
+int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, void* out, int out_dtype, float* scale, int dtype, int M, int K,
+                               int act, void* stream) {
+  std::lock_guard<std::mutex> lk(g_mutex);
+  int rc = NNCV_B200_OK;
+  if (!gate || !out || M < 0 || K <= 0 || dtype < 0 || dtype > 2 || act < 0 || act > 5) return fail(NNCV_B200_EINVAL, "gated_activation: bad argument");
+  if (ld == 0) ld = K;
+  if (ld < K) return fail(NNCV_B200_EINVAL, "gated_activation: ld is less than K");
+  if (!of_type(gate, dtype) || !of_type(up, dtype)) return fail(NNCV_B200_EINVAL, "gated_activation: a pointer is not on its type's boundary");
+  if ((rc = check_out("gated_activation", out_dtype, dtype, out, scale))) return rc;
+  if ((out == gate || out == up) && (ld != K || out_dtype == NNCV_B200_E4M3))
+    return fail(NNCV_B200_EINVAL, "gated_activation: the result may take the place of gate or up only where ld is K and the types agree");
+  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  GatedArgs a;
+  a.gate = gate; a.up = up; a.ld = ld; a.out = out; a.scale = scale; a.dtype = (DType)dtype; a.to_e4m3 = out_dtype == NNCV_B200_E4M3;
+  a.M = M; a.K = K; a.act = act; a.sm_count = g_dev.sm_count;
+  LAUNCH(launch_gated_activation(a, (cudaStream_t)stream));
+  return ok();
+}
+
+int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, float* scale, int M, int K, int block_rows, void* stream) {
+  std::lock_guard<std::mutex> lk(g_mutex);
+  int rc = NNCV_B200_OK;
+  if (!x || !q || !scale || M < 0 || K <= 0 || dtype < 0 || dtype > 2) return fail(NNCV_B200_EINVAL, "quantize_e4m3: bad argument");
+  if (block_rows != 1 && block_rows != 128) return fail(NNCV_B200_EINVAL, "quantize_e4m3: block_rows must be 1 or 128");
+  if (ldx == 0) ldx = K;
+  if (ldx < K) return fail(NNCV_B200_EINVAL, "quantize_e4m3: ldx is less than K");
+  if (!of_type(x, dtype) || !on_boundary(scale, 4)) return fail(NNCV_B200_EINVAL, "quantize_e4m3: a pointer is not on its type's boundary");
+  if (q == x) return fail(NNCV_B200_EINVAL, "quantize_e4m3: q needs memory of its own");
+  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  if (block_rows == 128) {
+    LAUNCH(launch_quantize_blocks(x, ldx, (DType)dtype, q, scale, M, K, (cudaStream_t)stream));
+    return ok();
+  }
+  GatedArgs a;
+  a.gate = x; a.ld = ldx; a.out = q; a.scale = scale; a.dtype = (DType)dtype; a.to_e4m3 = true; a.M = M; a.K = K; a.sm_count = g_dev.sm_count;
+  LAUNCH(launch_gated_activation(a, (cudaStream_t)stream));
+  return ok();
+}
+
+int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, const float* scale_b, void* C, int M, int N, int K, int c_dtype,
+                          const float* bias, int relu, void* stream) {
+  std::lock_guard<std::mutex> lk(g_mutex);
+  int rc = NNCV_B200_OK;
+  if (!A || !scale_a || !B || !scale_b || !C || M < 0 || N <= 0 || K <= 0) return fail(NNCV_B200_EINVAL, "matmul_e4m3: bad argument");
+  if (c_dtype < 0 || c_dtype > 2) return fail(NNCV_B200_EINVAL, "matmul_e4m3: c_dtype must be F32, F16 or BF16");
+  if (K % 16 != 0) return fail(NNCV_B200_EINVAL, "matmul_e4m3: K must be a multiple of 16");
+  if (!on_boundary(A, 16) || !on_boundary(B, 16)) return fail(NNCV_B200_EINVAL, "matmul_e4m3: A and B must lie on 16-byte boundaries");
+  if (!of_type(C, c_dtype) || !on_boundary(scale_a, 4) || !on_boundary(scale_b, 4) || !on_boundary(bias, 4))
+    return fail(NNCV_B200_EINVAL, "matmul_e4m3: a pointer is not on its type's boundary");
+  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  GemmE4m3Args a;
+  a.A = A; a.scale_a = scale_a; a.B = B; a.scale_b = scale_b; a.C = C; a.bias = bias; a.c_dtype = (DType)c_dtype; a.relu = relu;
+  a.M = M; a.N = N; a.K = K; a.sm_count = g_dev.sm_count; a.error_flag = g_dev.error_flag;
+  LAUNCH(launch_gemm_e4m3(a, (cudaStream_t)stream));
+  return ok();
+}
+
 }  // extern "C"
