@@ -359,7 +359,7 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
  * address of an element are allowed; K a multiple of 8 with everything on 16-byte boundaries is read 16 bytes at a time.
  *
  * Root-mean-square norm of x, or of h = x + residual: out = h / sqrt(mean(h^2) + eps) * weight.
- *   x [M,K] of dtype; residual [M,K] of dtype or NULL; weight fp32 [K] or NULL (= 1); K up to 32768
+ *   x [M,K] of dtype; residual [M,K] of dtype or NULL; weight fp32 [K] or NULL (= 1)
  *   sum: NULL, or [M,K] of dtype that receives h (the norm is taken of h before this rounding); may be residual, or x where ldx is K
  *   out: [M,K] of out_dtype, which is dtype or NNCV_B200_E4M3; scale: fp32 [M, ceil(K/128)] with E4M3, else NULL
  * out may be x (where ldx is K) or residual, if it has their type. */

@@ -296,7 +296,6 @@ cudaError_t launch_concat(const void* const* in, const int* channels, int n_in, 
 cudaError_t launch_upsample2x(const void* in, void* out, DType dt, int N, int H, int W, int C, cudaStream_t st);
 
 // ---- a linear layer in 8 bits: e4m3 values with an fp32 scale for every block of 128 (value = q * scale) ----
-constexpr int kRmsNormMaxK = 32768;    // a row stays in the registers of one CTA
 struct RmsNormArgs {
   const void* x = nullptr;             // [M,K], rows ldx elements apart
   long long ldx = 0;
@@ -309,6 +308,7 @@ struct RmsNormArgs {
   DType dtype = kF16;
   bool to_e4m3 = false;
   int M = 0, K = 0;
+  int sm_count = 0;
 };
 cudaError_t launch_rmsnorm(const RmsNormArgs& a, cudaStream_t st);
 struct GatedArgs {

@@ -4,46 +4,71 @@
 // A block of values y:  s = max(largest finite |y|, 2^-100) / 448,  q = y / s rounded to e4m3 (448 is its largest value).
 // The least scale keeps 1 / s finite for a block of zeros.  What is not finite becomes NaN -- e4m3 has no infinity -- and leaves
 // the other values of its block as they are.
+//
+// All of it is bound by HBM.  Eight threads hold the 128 columns of a block: each has 16 of them, in two pieces of eight that lie 64
+// columns apart, so that what the eight load and store at once lies in a row.
 #include "activation.cuh"
+#include "epilogue.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
 
 namespace nncv_b200 {
 namespace {
 
-constexpr int kV = 8;             // values a thread holds of a row at a time; sixteen threads hold a block
+constexpr int kV = 16;            // values a thread holds of a block
+constexpr int kLanes = 8;         // threads that hold a block
 constexpr int kGroup = 128;
 constexpr float kTop = 448.0f, kLeast = 0x1p-100f;
 
-// Eight consecutive values from column `col` of a row of K.  VEC: the row is on a 16-byte boundary and K a multiple of 8.
+constexpr int kPiece = 8;         // consecutive values
+__device__ __forceinline__ int piece_col(int i, int t) { return (i * kLanes + t) * kPiece; }
+
+// What a thread has of a row, as it lies in memory.  VEC: pieces are on 16-byte boundaries and K holds whole ones.
+template <typename T> struct Raw {
+  static constexpr int kWords = (int)sizeof(T) * kPiece / 16;
+  uint4 p[kV / kPiece][kWords];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int col, int K, float (&v)[kV]) {
-  if (VEC) {
-    alignas(16) T raw[kV];
+__device__ __forceinline__ void load_raw(const T* row, int col0, int t, int K, Raw<T>& r) {
 #pragma unroll
-    for (int i = 0; i < (int)(kV * sizeof(T) / 16); ++i)
-      reinterpret_cast<uint4*>(raw)[i] = col < K ? *reinterpret_cast<const uint4*>(row + col + i * (16 / sizeof(T))) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kV / kPiece; ++i) {
+    const int col = col0 + piece_col(i, t);
+    if (VEC) {
 #pragma unroll
-    for (int e = 0; e < kV; ++e) v[e] = ef<T>(raw[e]);
-  } else {
+      for (int j = 0; j < Raw<T>::kWords; ++j) r.p[i][j] = col < K ? reinterpret_cast<const uint4*>(row + col)[j] : make_uint4(0, 0, 0, 0);
+    } else {
+      alignas(16) T e[kPiece];
 #pragma unroll
-    for (int e = 0; e < kV; ++e) v[e] = col + e < K ? ef<T>(row[col + e]) : 0.0f;
+      for (int j = 0; j < kPiece; ++j) e[j] = col + j < K ? row[col + j] : et<T>(0.0f);
+#pragma unroll
+      for (int j = 0; j < Raw<T>::kWords; ++j) r.p[i][j] = reinterpret_cast<const uint4*>(e)[j];
+    }
   }
 }
+template <typename T>
+__device__ __forceinline__ void to_float(const Raw<T>& r, float (&v)[kV]) {
+  const T* e = reinterpret_cast<const T*>(r.p);
+#pragma unroll
+  for (int i = 0; i < kV; ++i) v[i] = ef<T>(e[i]);
+}
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int col, int K, const float (&v)[kV]) {
-  if (VEC) {
-    if (col >= K) return;
-    alignas(16) T raw[kV];
+__device__ __forceinline__ void store_row(T* row, int col0, int t, int K, const float (&v)[kV]) {
 #pragma unroll
-    for (int e = 0; e < kV; ++e) raw[e] = et<T>(v[e]);
+  for (int i = 0; i < kV / kPiece; ++i) {
+    const int col = col0 + piece_col(i, t);
+    alignas(16) T e[kPiece];
 #pragma unroll
-    for (int i = 0; i < (int)(kV * sizeof(T) / 16); ++i)
-      *reinterpret_cast<uint4*>(row + col + i * (16 / sizeof(T))) = reinterpret_cast<const uint4*>(raw)[i];
-  } else {
+    for (int j = 0; j < kPiece; ++j) e[j] = et<T>(v[i * kPiece + j]);
+    if (VEC) {
+      if (col < K) {
 #pragma unroll
-    for (int e = 0; e < kV; ++e)
-      if (col + e < K) row[col + e] = et<T>(v[e]);
+        for (int j = 0; j < Raw<T>::kWords; ++j) reinterpret_cast<uint4*>(row + col)[j] = reinterpret_cast<const uint4*>(e)[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPiece; ++j)
+        if (col + j < K) row[col + j] = e[j];
+    }
   }
 }
 
@@ -51,212 +76,336 @@ __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a < INFINITY ? a : 0.0f;   // a NaN compares false
 }
+template <int LANES>
+__device__ __forceinline__ float max_of(float a) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  return a;
+}
+__device__ __forceinline__ float largest(const float (&v)[kV]) {   // NaN is passed over
+  float a = fabsf(v[0]);
+#pragma unroll
+  for (int e = 1; e < kV; ++e) a = fmaxf(a, fabsf(v[e]));
+  return a;
+}
+__device__ __forceinline__ float largest_finite(const float (&v)[kV]) {
+  float a = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) a = fmaxf(a, finite_abs(v[e]));
+  return a;
+}
+__device__ __forceinline__ void infinite_to_nan(float (&v)[kV]) {   // the conversion alone would make them 448
+#pragma unroll
+  for (int e = 0; e < kV; ++e) v[e] = fabsf(v[e]) < INFINITY ? v[e] : __int_as_float(0x7fffffff);
+}
 __device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax, kLeast) * (1.0f / kTop); }
-
-// Two values times 1 / s as e4m3; infinities become NaN (the conversion alone would make them 448).
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi, float inv) {
-  const float nan = __int_as_float(0x7fffffff);
-  lo = fabsf(lo) < INFINITY ? lo * inv : nan;
-  hi = fabsf(hi) < INFINITY ? hi * inv : nan;
+__device__ __forceinline__ float reciprocal(float s) {   // a step of fp32 off at most where 1 / s is a normal number
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
 template <bool VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ row, int col, int K, const float (&v)[kV], float inv) {
-  uint32_t h[4];
+__device__ __forceinline__ void store_e4m3(uint8_t* row, int col0, int t, int K, const float (&v)[kV], float inv) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = e4m3x2(v[2 * e], v[2 * e + 1], inv);
-  if (VEC) {
-    if (col < K) *reinterpret_cast<uint2*>(row + col) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-  } else {
+  for (int i = 0; i < kV / kPiece; ++i) {
+    const int col = col0 + piece_col(i, t);
+    uint32_t h[2];
 #pragma unroll
-    for (int e = 0; e < kV; ++e)
-      if (col + e < K) row[col + e] = (uint8_t)(h[e >> 1] >> (8 * (e & 1)));
+    for (int j = 0; j < 2; ++j) {
+      const float* q = v + i * kPiece + 4 * j;
+      h[j] = e4m3x2(q[0] * inv, q[1] * inv) | e4m3x2(q[2] * inv, q[3] * inv) << 16;
+    }
+    if (VEC) {
+      if (col < K) *reinterpret_cast<uint2*>(row + col) = make_uint2(h[0], h[1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPiece; ++j)
+        if (col + j < K) row[col + j] = (uint8_t)(h[j >> 2] >> (8 * (j & 3)));
+    }
   }
 }
 
-// Writes the block that these sixteen threads hold and its scale.
+// Writes the block that these eight threads hold and its scale.  Infinities are looked for only where one is the largest
+// value of some block of the warp: tested per element they took a third of the instructions.
 template <bool VEC>
-__device__ __forceinline__ void put_group(uint8_t* __restrict__ row, float* __restrict__ scales, int col, int K, const float (&v)[kV]) {
-  float amax = 0.0f;
-#pragma unroll
-  for (int e = 0; e < kV; ++e) amax = fmaxf(amax, finite_abs(v[e]));
-#pragma unroll
-  for (int o = 8; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+__device__ __forceinline__ void put_block(uint8_t* row, float* scale, int col0, int t, int K, float (&v)[kV]) {
+  float amax = max_of<kLanes>(largest(v));
+  if (__any_sync(0xffffffffu, !(amax < INFINITY))) {
+    amax = max_of<kLanes>(largest_finite(v));
+    infinite_to_nan(v);
+  }
   const float s = block_scale(amax);
-  store_e4m3<VEC>(row, col, K, v, 1.0f / s);
-  if (col < K && col % kGroup == 0) scales[col / kGroup] = s;
+  store_e4m3<VEC>(row, col0, t, K, v, reciprocal(s));
+  if (t == 0 && col0 < K) *scale = s;
+}
+
+// x / (1 + exp(-x)) on the hardware's exponential and reciprocal: exp is off by 2 steps of fp32 and by what rounding x * log2(e) makes of
+// it, far below half a step of the 16-bit values that come in.  exp(-x) = inf gives 0, or NaN for -inf, as the quotient does.
+__device__ __forceinline__ float silu16(float x) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  return x * reciprocal(1.0f + e);
 }
 
 // ---------------------------------------------------------------- root-mean-square norm ----
-// One CTA a row; the row stays in registers between the sum of squares and the result, so every tensor is read once.
-template <typename T, bool VEC, bool Q, int ITER>
-__global__ void __launch_bounds__(ITER <= 2 ? 1024 : 512)
-rmsnorm_kernel(const T* x, long long ldx, const T* residual, const float* __restrict__ weight, float eps, T* sum, void* out,
-                               float* scale, int K) {
-  __shared__ float s_part[32];
+// The sum of a value over the CTA, in every thread; `part`: 32 floats of shared memory that nobody reads or writes meanwhile.
+__device__ __forceinline__ float cta_sum(float v, float* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0) part[warp] = v;
+  __syncthreads();
+  v = lane < (int)(blockDim.x >> 5) ? part[lane] : 0.0f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void add_raw(const Raw<T>& r, float (&h)[kV]) {
+  float v[kV];
+  to_float<T>(r, v);
+#pragma unroll
+  for (int e = 0; e < kV; ++e) h[e] += v[e];
+}
+template <bool VEC>
+__device__ __forceinline__ void load_weight(const float* weight, int col0, int t, int K, float (&w)[kV]) {
+  if (weight) {
+    Raw<float> r;
+    load_raw<float, VEC>(weight, col0, t, K, r);
+    to_float<float>(r, w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kV; ++e) w[e] = 1.0f;
+  }
+}
+
+// Rows of up to kAheadK: a CTA takes one row after the other, which stays in registers between the sum of squares and the result, so
+// that every tensor is read once; the next row is on its way while this one is worked on, and the weights stay in registers.
+// (With a CTA a row, loads were under way only in the first half of its life: 4096 x 4096 bf16 with residual to e4m3 23.5 us, now 19.8:
+// 5.9 TB/s.)
+constexpr int kAheadK = 16384;
+template <typename T, bool VEC, bool Q, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 2 : 1)
+rmsnorm_kernel(const T* x, long long ldx, const T* residual, const float* weight, float eps, T* sum, void* out, float* scale, int M, int K) {
+  __shared__ float s_part[2][32];
+  const int t = threadIdx.x & (kLanes - 1), col0 = (int)threadIdx.x / kLanes * kGroup, kb = (K + kGroup - 1) / kGroup;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
+  Raw<T> a, b;
+  auto load = [&](long long row) {
+    load_raw<T, VEC>(x + row * ldx, col0, t, K, a);
+    if (residual) load_raw<T, VEC>(residual + row * K, col0, t, K, b);
+  };
+  constexpr bool kKeep = THREADS < 512;   // with 64 registers a thread the weights come from L1 for every row
+  float w[kV];
+  if (kKeep) load_weight<VEC>(weight, col0, t, K, w);
+  load(blockIdx.x);
+  uint32_t turn = 0;   // the other half of s_part is written next: whoever reads this one is past the barrier of the row before
+  for (long long row = blockIdx.x; row < M; row += gridDim.x, turn ^= 1u) {
+    float h[kV], ss = 0.0f;
+    to_float<T>(a, h);
+    if (residual) add_raw<T>(b, h);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) ss = fmaf(h[e], h[e], ss);
+    if (row + gridDim.x < M) load(row + gridDim.x);
+    if (sum) store_row<T, VEC>(sum + row * K, col0, t, K, h);
+    const float norm = 1.0f / sqrtf(cta_sum(ss, s_part[turn]) / (float)K + eps);
+    if (!kKeep) load_weight<VEC>(weight, col0, t, K, w);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) h[e] *= norm * w[e];
+    if (Q) put_block<VEC>(static_cast<uint8_t*>(out) + row * K, scale + row * kb + col0 / kGroup, col0, t, K, h);
+    else store_row<T, VEC>(static_cast<T*>(out) + row * K, col0, t, K, h);
+  }
+}
+
+// Longer rows are read twice, the second time from L2.  `sum` is written in the second pass, so that it may take the place of x
+// or the residual.
+constexpr int kLongThreads = 512;
+template <typename T, bool VEC, bool Q>
+__global__ void __launch_bounds__(kLongThreads)
+rmsnorm_long_kernel(const T* x, long long ldx, const T* residual, const float* weight, float eps, T* sum, void* out, float* scale, int K) {
+  __shared__ float s_part[32];
+  const int t = threadIdx.x & (kLanes - 1), first = (int)threadIdx.x / kLanes * kGroup, step = kLongThreads / kLanes * kGroup, kb = (K + kGroup - 1) / kGroup;
   const long long row = blockIdx.x;
-  const int threads = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float h[ITER][kV];
-#pragma unroll
-  for (int i = 0; i < ITER; ++i) load8<T, VEC>(x + row * ldx, (i * threads + (int)threadIdx.x) * kV, K, h[i]);
-  if (residual) {
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      float r[kV];
-      load8<T, VEC>(residual + row * K, (i * threads + (int)threadIdx.x) * kV, K, r);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) h[i][e] += r[e];
-    }
-  }
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   float ss = 0.0f;
+  for (int col0 = first; col0 < K; col0 += step) {
+    Raw<T> a, b;
+    load_raw<T, VEC>(x + row * ldx, col0, t, K, a);
+    if (residual) load_raw<T, VEC>(residual + row * K, col0, t, K, b);
+    float h[kV];
+    to_float<T>(a, h);
+    if (residual) add_raw<T>(b, h);
+    float part = 0.0f;
 #pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    if (sum) store8<T, VEC>(sum + row * K, (i * threads + (int)threadIdx.x) * kV, K, h[i]);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+    for (int e = 0; e < kV; ++e) part = fmaf(h[e], h[e], part);
+    ss += part;
   }
+  const float norm = 1.0f / sqrtf(cta_sum(ss, s_part) / (float)K + eps);
+  for (int base = 0; base < K; base += step) {   // the same number of rounds for every thread: a block's threads exchange its maximum
+    const int col0 = base + first;
+    Raw<T> a, b;
+    load_raw<T, VEC>(x + row * ldx, col0, t, K, a);
+    if (residual) load_raw<T, VEC>(residual + row * K, col0, t, K, b);
+    float h[kV], w[kV];
+    load_weight<VEC>(weight, col0, t, K, w);
+    to_float<T>(a, h);
+    if (residual) add_raw<T>(b, h);
+    if (sum) store_row<T, VEC>(sum + row * K, col0, t, K, h);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (lane == 0) s_part[warp] = ss;
-  __syncthreads();
-  float total = lane < (threads >> 5) ? s_part[lane] : 0.0f;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const float norm = 1.0f / sqrtf(total / (float)K + eps);
-#pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int col = (i * threads + (int)threadIdx.x) * kV;
-    float w[kV];
-    if (weight) load8<float, VEC>(weight, col, K, w);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) h[i][e] = weight ? h[i][e] * norm * w[e] : h[i][e] * norm;
-    if (Q) put_group<VEC>(static_cast<uint8_t*>(out) + row * K, scale + row * ((K + kGroup - 1) / kGroup), col, K, h[i]);
-    else store8<T, VEC>(static_cast<T*>(out) + row * K, col, K, h[i]);
+    for (int e = 0; e < kV; ++e) h[e] *= norm * w[e];
+    if (Q) put_block<VEC>(static_cast<uint8_t*>(out) + row * K, scale + row * kb + col0 / kGroup, col0, t, K, h);
+    else store_row<T, VEC>(static_cast<T*>(out) + row * K, col0, t, K, h);
   }
 }
 
 // ---------------------------------------------------------------- (gated) activation -------
-// Sixteen threads a block of 128 columns of a row; gate * 1 where there is no `up`.
-template <typename T, bool VEC, bool Q>
-__global__ void __launch_bounds__(256) gated_kernel(const T* gate, const T* up, long long ld, void* out,
-                                                    float* __restrict__ scale, long long groups, int kb, int K, int act) {
+// A thread has its part of one block at a time, of two where there is a single tensor: then as many bytes are under way.  ACT: the
+// activation, or -1 for the one in `act`.
+constexpr int kGatedThreads = 256, kGatedBlocks = kGatedThreads / kLanes;
+template <typename T, bool VEC, bool Q, bool UP, int ACT>
+__global__ void __launch_bounds__(kGatedThreads) gated_kernel(const T* gate, const T* up, long long ld, void* out, float* scale, uint32_t blocks,
+                                                              epi::FastDiv kb, int K, int act) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long step = (long long)gridDim.x * (blockDim.x / 16);
-  for (long long g0 = (long long)blockIdx.x * (blockDim.x / 16); g0 < groups; g0 += step) {
-    const long long g = g0 + threadIdx.x / 16;
-    const bool in = g < groups;
-    const long long row = in ? g / kb : 0;
-    const int col = in ? (int)(g - row * kb) * kGroup + (int)(threadIdx.x & 15) * kV : K;
+  constexpr int kUnroll = UP ? 1 : 2;
+  const int t = threadIdx.x & (kLanes - 1);
+  const uint32_t first = blockIdx.x * (kGatedBlocks * kUnroll) + threadIdx.x / kLanes;
+  Raw<T> g[kUnroll], u[kUnroll];
+  long long row[kUnroll];
+  int col0[kUnroll];
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    const uint32_t b = first + i * kGatedBlocks, r = epi::div_by(b, kb);
+    row[i] = b < blocks ? r : 0;
+    col0[i] = b < blocks ? (int)(b - r * kb.d) * kGroup : K;
+    load_raw<T, VEC>(gate + row[i] * ld, col0[i], t, K, g[i]);
+    if (UP) load_raw<T, VEC>(up + row[i] * ld, col0[i], t, K, u[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
     float v[kV];
-    load8<T, VEC>(gate + row * ld, col, K, v);
+    to_float<T>(g[i], v);
 #pragma unroll
-    for (int e = 0; e < kV; ++e) v[e] = activate<sizeof(T) == 2>(v[e], act);
-    if (up) {
-      float u[kV];
-      load8<T, VEC>(up + row * ld, col, K, u);
+    for (int e = 0; e < kV; ++e) v[e] = ACT == kActSilu && sizeof(T) == 2 ? silu16(v[e]) : activate<sizeof(T) == 2>(v[e], ACT < 0 ? act : ACT);
+    if (UP) {
+      float w[kV];
+      to_float<T>(u[i], w);
 #pragma unroll
-      for (int e = 0; e < kV; ++e) v[e] *= u[e];
+      for (int e = 0; e < kV; ++e) v[e] *= w[e];
     }
-    if (!VEC) {   // what an activation makes of the zeros behind the row is not part of its block
+    if (Q) {
+      if (ACT != kActNone && ACT != kActSilu && !UP) {   // what the activation makes of the zeros behind the row is not part of its block
 #pragma unroll
-      for (int e = 0; e < kV; ++e) v[e] = col + e < K ? v[e] : 0.0f;
-    } else if (col >= K) {
-#pragma unroll
-      for (int e = 0; e < kV; ++e) v[e] = 0.0f;
+        for (int e = 0; e < kV; ++e)
+          if (col0[i] + piece_col(e / kPiece, t) + e % kPiece >= K) v[e] = 0.0f;
+      }
+      put_block<VEC>(static_cast<uint8_t*>(out) + row[i] * K, scale + row[i] * kb.d + col0[i] / kGroup, col0[i], t, K, v);
+    } else {
+      store_row<T, VEC>(static_cast<T*>(out) + row[i] * K, col0[i], t, K, v);
     }
-    if (Q) put_group<VEC>(static_cast<uint8_t*>(out) + row * K, scale + row * kb, col, K, v);
-    else store8<T, VEC>(static_cast<T*>(out) + row * K, col, K, v);
   }
 }
 
 // ---------------------------------------------------------------- blocks of 128 x 128 ------
-// One CTA a block, which stays in registers between its largest value and the result: 16 threads a row of 128, 16 rows at a time.
-constexpr int kBlockIter = kGroup / 16;
+// One CTA a block, which stays in registers between its largest value and the result: kBlockThreads / 8 rows at a time.
+constexpr int kBlockThreads = 256, kBlockRows = kBlockThreads / kLanes, kBlockIter = kGroup / kBlockRows;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_block_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
-                                                             float* __restrict__ scale, int M, int K) {
-  __shared__ float s_part[8];
+__global__ void __launch_bounds__(kBlockThreads) quantize_block_kernel(const T* x, long long ldx, uint8_t* q, float* scale, int M, int K) {
+  __shared__ float s_part[kBlockThreads / 32];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const int kb = (K + kGroup - 1) / kGroup, bm = (int)(blockIdx.x / kb), bk = (int)(blockIdx.x % kb);
-  const int col = bk * kGroup + (int)(threadIdx.x & 15) * kV;
-  float v[kBlockIter][kV];
-  float amax = 0.0f;
+  const int kb = (K + kGroup - 1) / kGroup, bm = (int)(blockIdx.x / kb), col0 = (int)(blockIdx.x % kb) * kGroup;
+  const int t = threadIdx.x & (kLanes - 1), r0 = bm * kGroup + (int)(threadIdx.x / kLanes);
+  Raw<T> raw[kBlockIter];
+#pragma unroll
+  for (int i = 0; i < kBlockIter; ++i) load_raw<T, VEC>(x + (long long)(r0 + i * kBlockRows) * ldx, r0 + i * kBlockRows < M ? col0 : K, t, K, raw[i]);
+  float v[kBlockIter][kV], amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < kBlockIter; ++i) {
-    const int row = bm * kGroup + i * 16 + (int)(threadIdx.x >> 4);
-    load8<T, VEC>(x + (long long)row * ldx, row < M ? col : K, K, v[i]);
+    to_float<T>(raw[i], v[i]);
+    amax = fmaxf(amax, largest(v[i]));
   }
+  if (__syncthreads_or(!(amax < INFINITY))) {
+    amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kBlockIter; ++i)
-#pragma unroll
-    for (int e = 0; e < kV; ++e) amax = fmaxf(amax, finite_abs(v[i][e]));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int i = 0; i < kBlockIter; ++i) {
+      amax = fmaxf(amax, largest_finite(v[i]));
+      infinite_to_nan(v[i]);
+    }
+  }
+  amax = max_of<32>(amax);
   if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = amax;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, s_part[i]);
-  const float s = block_scale(amax), inv = 1.0f / s;
+  for (int i = 0; i < kBlockThreads / 32; ++i) amax = fmaxf(amax, s_part[i]);
+  const float s = block_scale(amax), inv = reciprocal(s);
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
 #pragma unroll
   for (int i = 0; i < kBlockIter; ++i) {
-    const int row = bm * kGroup + i * 16 + (int)(threadIdx.x >> 4);
-    if (row < M) store_e4m3<VEC>(q + (long long)row * K, col, K, v[i], inv);
+    const int row = r0 + i * kBlockRows;
+    if (row < M) store_e4m3<VEC>(q + (long long)row * K, col0, t, K, v[i], inv);
   }
 }
 
 inline bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+// Rows of x in whole pieces on 16-byte boundaries.
+template <typename T>
+bool pieces(const void* x, long long ld, int K) { return K % kPiece == 0 && ld * (long long)sizeof(T) % 16 == 0 && aligned(x, 16); }
 
 template <typename T, bool VEC, bool Q>
 cudaError_t rmsnorm_as(const RmsNormArgs& a, cudaStream_t st) {
-  const int chunks = (a.K + kV - 1) / kV;
-  const int iter = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 8;
-  const int threads = ((chunks + iter - 1) / iter + 31) / 32 * 32;
-#define NNCV_NORM(I_)                                                                                                                        \
-  if (iter == I_)                                                                                                                            \
-    return launch_pdl(rmsnorm_kernel<T, VEC, Q, I_>, dim3((unsigned)a.M), dim3(threads), 0, st, static_cast<const T*>(a.x), a.ldx,           \
+  if (a.K > kAheadK)
+    return launch_pdl(rmsnorm_long_kernel<T, VEC, Q>, dim3((unsigned)a.M), dim3(kLongThreads), 0, st, static_cast<const T*>(a.x), a.ldx,
                       static_cast<const T*>(a.residual), a.weight, a.eps, static_cast<T*>(a.sum), a.out, a.scale, a.K);
-  NNCV_NORM(1) NNCV_NORM(2) NNCV_NORM(8)
-#undef NNCV_NORM
-  return cudaErrorInvalidValue;
+  const int threads = ((a.K + kGroup - 1) / kGroup * kLanes + 31) / 32 * 32;
+  // as many CTAs as find room at once: 768 threads an SM with 80 registers each (4096 x 4096: 512 23.9 us, 768 19.8, 1280 21.2), 1024 with 64
+  auto kern = threads <= 384 ? rmsnorm_kernel<T, VEC, Q, 384> : threads <= 512 ? rmsnorm_kernel<T, VEC, Q, 512> : rmsnorm_kernel<T, VEC, Q, 1024>;
+  const long long grid = (long long)(a.sm_count > 0 ? a.sm_count : 148) * (threads <= 384 ? 768 / threads : 1024 / threads);
+  return launch_pdl(kern, dim3((unsigned)(grid < a.M ? grid : a.M)), dim3(threads), 0, st, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.residual),
+                    a.weight, a.eps, static_cast<T*>(a.sum), a.out, a.scale, a.M, a.K);
 }
 template <typename T>
 cudaError_t rmsnorm_of(const RmsNormArgs& a, cudaStream_t st) {
-  const bool vec = a.K % kV == 0 && a.ldx * (long long)sizeof(T) % 16 == 0 && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) &&
-                   aligned(a.sum, 16) && aligned(a.out, a.to_e4m3 ? 8 : 16);
+  const bool vec = pieces<T>(a.x, a.ldx, a.K) && aligned(a.residual, 16) && aligned(a.weight, 16) && aligned(a.sum, 16) && aligned(a.out, a.to_e4m3 ? kPiece : 16);
   if (a.to_e4m3) return vec ? rmsnorm_as<T, true, true>(a, st) : rmsnorm_as<T, false, true>(a, st);
   return vec ? rmsnorm_as<T, true, false>(a, st) : rmsnorm_as<T, false, false>(a, st);
 }
 
+template <typename T, bool VEC, bool Q>
+cudaError_t gated_as(const GatedArgs& a, cudaStream_t st) {
+  const int kb = (a.K + kGroup - 1) / kGroup;
+  const long long blocks = (long long)a.M * kb, each = kGatedBlocks * (a.up ? 1 : 2);
+  if (blocks > 0x7fffffffLL - each) return cudaErrorInvalidValue;
+  auto kern = a.up ? (a.act == kActSilu ? gated_kernel<T, VEC, Q, true, kActSilu> : gated_kernel<T, VEC, Q, true, -1>)
+                   : (a.act == kActNone ? gated_kernel<T, VEC, Q, false, kActNone> : gated_kernel<T, VEC, Q, false, -1>);
+  return launch_pdl(kern, dim3((unsigned)((blocks + each - 1) / each)), dim3(kGatedThreads), 0, st,
+                    static_cast<const T*>(a.gate), static_cast<const T*>(a.up), a.ld, a.out, a.scale, (uint32_t)blocks, epi::fast_div((uint32_t)kb), a.K, a.act);
+}
 template <typename T>
 cudaError_t gated_of(const GatedArgs& a, cudaStream_t st) {
-  const bool vec = a.K % kV == 0 && a.ld * (long long)sizeof(T) % 16 == 0 && aligned(a.gate, 16) && aligned(a.up, 16) && aligned(a.out, a.to_e4m3 ? 8 : 16);
-  const int kb = (a.K + kGroup - 1) / kGroup;
-  const long long groups = (long long)a.M * kb, most = (long long)(a.sm_count > 0 ? a.sm_count : 148) * 8;
-  const long long need = (groups + 15) / 16;
-  auto kern = a.to_e4m3 ? (vec ? gated_kernel<T, true, true> : gated_kernel<T, false, true>) : (vec ? gated_kernel<T, true, false> : gated_kernel<T, false, false>);
-  return launch_pdl(kern, dim3((unsigned)(need < most ? need : most)), dim3(256), 0, st, static_cast<const T*>(a.gate), static_cast<const T*>(a.up), a.ld, a.out,
-                    a.scale, groups, kb, a.K, a.act);
+  const bool vec = pieces<T>(a.gate, a.ld, a.K) && aligned(a.up, 16) && aligned(a.out, a.to_e4m3 ? kPiece : 16);
+  if (a.to_e4m3) return vec ? gated_as<T, true, true>(a, st) : gated_as<T, false, true>(a, st);
+  return vec ? gated_as<T, true, false>(a, st) : gated_as<T, false, false>(a, st);
 }
 
 template <typename T>
 cudaError_t quantize_blocks_of(const T* x, long long ldx, uint8_t* q, float* scale, int M, int K, cudaStream_t st) {
-  const bool vec = K % kV == 0 && ldx * (long long)sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(q, 8);
+  const bool vec = pieces<T>(x, ldx, K) && aligned(q, kPiece);
   const long long blocks = (long long)((M + kGroup - 1) / kGroup) * ((K + kGroup - 1) / kGroup);
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  return launch_pdl(vec ? quantize_block_kernel<T, true> : quantize_block_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, st, x, ldx, q, scale, M, K);
+  return launch_pdl(vec ? quantize_block_kernel<T, true> : quantize_block_kernel<T, false>, dim3((unsigned)blocks), dim3(kBlockThreads), 0, st, x, ldx, q, scale, M, K);
 }
 
 }  // namespace
 
 cudaError_t launch_rmsnorm(const RmsNormArgs& a, cudaStream_t st) {
-  if (a.K > kRmsNormMaxK) return cudaErrorInvalidValue;
   return a.dtype == kF32 ? rmsnorm_of<float>(a, st) : a.dtype == kF16 ? rmsnorm_of<__half>(a, st) : rmsnorm_of<__nv_bfloat16>(a, st);
 }
 

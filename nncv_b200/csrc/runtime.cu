@@ -3100,7 +3100,6 @@ int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const 
   std::lock_guard<std::mutex> lk(g_mutex);
   int rc = NNCV_B200_OK;
   if (!x || !out || M < 0 || K <= 0 || dtype < 0 || dtype > 2 || !(eps >= 0.0f)) return fail(NNCV_B200_EINVAL, "rmsnorm: bad argument");
-  if (K > kRmsNormMaxK) return fail(NNCV_B200_EINVAL, "rmsnorm: K may be at most %d", kRmsNormMaxK);
   if (ldx == 0) ldx = K;
   if (ldx < K) return fail(NNCV_B200_EINVAL, "rmsnorm: ldx is less than K");
   if (!of_type(x, dtype) || !of_type(residual, dtype) || !of_type(sum, dtype) || !on_boundary(weight, 4))
@@ -3111,7 +3110,7 @@ int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const 
   if ((rc = device_init()) || M == 0) return rc ? rc : ok();
   RmsNormArgs a;
   a.x = x; a.ldx = ldx; a.residual = residual; a.weight = (const float*)weight; a.eps = eps; a.sum = sum; a.out = out; a.scale = scale;
-  a.dtype = (DType)dtype; a.to_e4m3 = out_dtype == NNCV_B200_E4M3; a.M = M; a.K = K;
+  a.dtype = (DType)dtype; a.to_e4m3 = out_dtype == NNCV_B200_E4M3; a.M = M; a.K = K; a.sm_count = g_dev.sm_count;
   LAUNCH(launch_rmsnorm(a, (cudaStream_t)stream));
   return ok();
 }
