@@ -597,7 +597,7 @@ cudaError_t launch_as(const GemmE4m3Args& a, GeParams p, int splits, cudaStream_
   const size_t smem = smem_of<BN, PAIR>(a_rows, &p.stages);
   p.m_tiles = (a.M + kTileM - 1) / kTileM;
   p.n_tiles = (a.N + BN - 1) / BN;
-  if ((long long)p.m_tiles * p.n_tiles > 0x3fffffffLL || (long long)kGroupM * p.n_tiles > 0x3fffffffLL) return cudaErrorInvalidValue;
+  if ((long long)p.m_tiles * p.n_tiles > 0x3fffffffLL) return cudaErrorInvalidValue;
   p.div_band = epi::fast_div((uint32_t)(kGroupM * p.n_tiles));
   p.div_last = epi::fast_div((uint32_t)(p.m_tiles % kGroupM ? p.m_tiles % kGroupM : kGroupM));
   CUtensorMap tm_a, tm_b, tm_c = {};   // a result whose rows are not on 16-byte boundaries is written without a map

@@ -83,7 +83,19 @@ def test_matmul(m, n, k, cdt, epilogue):
     check_matmul(m, n, k, cdt, epilogue)
 
 
-@pytest.mark.parametrize("m,n,k,cdt,offset", [(3, 64, 128, F32, 1), (40, 264, 256, BF16, 1), (40, 264, 256, BF16, 2), (200, 1024, 256, F16, 4), (1, 2048, 512, BF16, 8)])
+@pytest.mark.parametrize("m,n,k", [
+    (2304, 2307, 1152), (2300, 2304, 1152),          # 256 x 128 on pairs
+    (1600, 1999, 2000), (1500, 2056, 2064),          # 256 x 256 on pairs
+    (777, 5000, 640), (776, 5001, 656),              # 128 x 128
+    (1, 5876, 2080), (9, 2999, 4096), (9, 3000, 4096), (1, 999, 2720),     # 128 x 128, two, four and eight CTAs a tile
+    (3, 4607, 2752), (40, 2050, 8192), (200, 129, 8192), (200, 128, 8192)])   # 128 x 64, likewise
+@pytest.mark.parametrize("cdt,epilogue", [(F32, True), (F16, False), (BF16, True), (F32, False)])
+def test_matmul_every_tile(m, n, k, cdt, epilogue):
+    """The sizes that the model gives to each tile and each number of CTAs, with and without rows on 16-byte boundaries."""
+    check_matmul(m, n, k, cdt, epilogue)
+
+
+@pytest.mark.parametrize("m,n,k,cdt,offset", [(1600, 2000, 2000, BF16, 1), (1600, 2000, 2000, F32, 2), (3, 64, 128, F32, 1), (40, 264, 256, BF16, 1), (40, 264, 256, BF16, 2), (200, 1024, 256, F16, 4), (1, 2048, 512, BF16, 8)])
 def test_matmul_into_any_address(m, n, k, cdt, offset):
     check_matmul(m, n, k, cdt, False, offset)
 
@@ -205,7 +217,7 @@ def check_norm(m, k, dt, e4m3, residual=True, weight=True, pad=0, offset=0, big=
 
 
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 8), (2, 7), (1, 4096), (3, 128), (5, 129), (7, 1000), (64, 1024), (33, 2047), (9, 5120), (4, 8192),
-                                 (2, 8200), (3, 16384), (2, 16392), (2, 32768), (1, 32767), (700, 512), (1025, 200)])
+                                 (2, 8200), (3, 16384), (2, 16392), (2, 32768), (1, 32767), (3, 40000), (300, 6144), (450, 12000), (700, 512), (1025, 200)])
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
 @pytest.mark.parametrize("e4m3", [True, False])
 def test_norm(m, k, dt, e4m3):
@@ -227,7 +239,7 @@ def test_norm_sizes_of_values():
 
 
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
-@pytest.mark.parametrize("k", [768, 771])
+@pytest.mark.parametrize("k", [768, 771, 9000, 16400, 16403])
 def test_norm_in_place(dt, k):
     g = gen(11, dt, k)
     x, r, w = norm_inputs(g, 50, k, dt, 0, 0, True, True, 1.0)
