@@ -27,7 +27,8 @@ constexpr int kMaxStages = 20, kMaxAccs = 4;
 constexpr size_t kSmemLimit = 226 * 1024;   // beside it a few hundred bytes of static shared memory
 constexpr int kGroupM = 8;                  // row tiles that are walked together with all column tiles: both operands' tiles stay in L2
 constexpr int kBufs = 2;                    // staging buffers of a warp, 32 rows of 128 bytes each
-constexpr int kScaleBytes = 4096;
+constexpr int kSlots = 16;                  // blocks whose products of scales are held
+constexpr int kScaleBytes = kSlots * (kBM + 4) * 8;
 
 constexpr int threads_of(int bn) { return bn == 64 ? 256 : 384; }
 
@@ -140,8 +141,9 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   constexpr uint32_t kTmemCols = kAccs * BN;
   constexpr int kNS = BN == 256 ? 2 : 1, kPartN = BN / kNS;    // column parts of an accumulator; a warp has 64 columns of each
   static_assert(kPartN == 16 * EW, "");
-  constexpr uint32_t kSlots = 2 * kAccs, kSlotBytes = kBM * kNS * 4;   // products of the scales of a block: of each row, for each part
-  static_assert(kSlots * kSlotBytes <= kScaleBytes, "");
+  // products of the scales of a block, of each row for each part; the lanes of a store (4 blocks x 8 rows) meet no bank twice
+  constexpr uint32_t kSlotBytes = (kBM + 4) * 4 * kNS;
+  static_assert(kSlots * kSlotBytes <= (uint32_t)kScaleBytes, "");
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_abort;
   __shared__ uint32_t s_tmem;
@@ -222,9 +224,9 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   ptx::grid_launch_dependents();
 
   // 256 x 256: 384 threads start with 168 registers each (64,512); the first four warps give up what the others take:
-  // 128 * 40 + 256 * 232 = 64,512
+  // 128 * 72 + 256 * 216 = 64,512
   if (warp < 4) {
-    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
       // ---------------------------------------------------------------- TMA producer ----
       const uint32_t issue = ptx::elect_one();
@@ -321,50 +323,62 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       }
     } else {
       // ---------------------------------------------------------------- scales ----------
-      // The products of the scales of every row (two a thread) go to shared memory a block or two ahead: with loads of its own
-      // an epilogue warp lost 70 clocks a block.  A slot was last read two rounds of the accumulators ago, and the MMAs of one
-      // round ago were not issued before that was over.
-      const int r0 = (warp - 2) * 32 + lane;
+      // The products of the scales of every row, for each part, go to shared memory: with loads of its own an epilogue warp lost 70 clocks a
+      // block.  They come for a chunk of blocks at once, a chunk ahead of their use (a row a lane and a block at a time, 32 sectors a
+      // load set the pace of the smaller tiles: 512 x 4096 x 4096 on 256 x 128 tiles 14.0 us, now 12.2).
+      // A chunk is written when its first block's turn has come: the MMAs of kAccs blocks ago are complete then, so they were issued, so
+      // block 2 kAccs ago, four or eight, has been read, while the slots written are those of 13 blocks ago and older.
+      constexpr int kChunk = 4, kRows = 32 / kChunk, kLoads = 64 / kRows;   // blocks and rows of a load (8 x 4: 0.3 us later at the first block)
+      const int k = lane & (kChunk - 1), r0 = (warp - 2) * 64 + lane / kChunk;
       uint32_t ac = 0, aph = 0, slot = 0;
       bool okw = true;
+      float v[kLoads], f0 = 0.0f, f1 = 0.0f;
+      auto fetch = [&](int m0, int n0, int kb) {
+        const float* sa = p.scale_a + (size_t)(m0 + r0) * p.KB + kb + k;
+        const float* sb = p.scale_b + (size_t)(n0 / kBlockK) * p.KB + kb + k;
+        const bool in = kb + k < kb_hi;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) v[j] = in && m0 + r0 + j * kRows < p.M ? __ldg(sa + (size_t)(j * kRows) * p.KB) : 0.0f;
+        f0 = in ? __ldg(sb) : 0.0f;
+        if (kNS == 2) f1 = in && n0 + kPartN < p.N ? __ldg(sb + p.KB) : 0.0f;
+      };
+      auto tell = [&]() {   // this warp's scales of the block are there
+        if (lane == 0) ptx::mbar_arrive(acc_full + 8 * ac);
+        if (++ac == kAccs) { ac = 0; aph ^= 1u; }
+        slot = (slot + 1) & (kSlots - 1);
+      };
       int m0, n0;
-      for (int i = 0; okw && item(i, m0, n0); ++i) {
-        const float* sa0 = p.scale_a + (size_t)(m0 + r0 < p.M ? m0 + r0 : 0) * p.KB;
-        const float* sa1 = p.scale_a + (size_t)(m0 + r0 + 64 < p.M ? m0 + r0 + 64 : 0) * p.KB;
-        const float* sb0 = p.scale_b + (size_t)(n0 < p.N ? n0 / kBlockK : 0) * p.KB;
-        const float* sb1 = kNS == 2 && n0 + kPartN < p.N ? sb0 + p.KB : sb0;
-        float a0 = 0.0f, a1 = 0.0f, b0 = 0.0f, b1 = 0.0f;
-        if (kb_lo < kb_hi) {
-          a0 = __ldg(sa0 + kb_lo); a1 = __ldg(sa1 + kb_lo); b0 = __ldg(sb0 + kb_lo);
-          if (kNS == 2) b1 = __ldg(sb1 + kb_lo);
-        }
-        for (int kb = kb_lo; kb < kb_hi; ++kb) {
-          const float x0 = a0 * b0, x1 = a1 * b0, y0 = a0 * b1, y1 = a1 * b1;
-          if (kb + 1 < kb_hi) {
-            a0 = __ldg(sa0 + kb + 1); a1 = __ldg(sa1 + kb + 1); b0 = __ldg(sb0 + kb + 1);
-            if (kNS == 2) b1 = __ldg(sb1 + kb + 1);
-          }
+      bool more = kb_lo < kb_hi && item(0, m0, n0);
+      if (more) fetch(m0, n0, kb_lo);
+      for (int i = 0; more && okw; ++i) {
+        int next_m0, next_n0;
+        more = item(i + 1, next_m0, next_n0);
+        for (int kb = kb_lo; kb < kb_hi && okw; kb += kChunk) {
           if (!ptx::warp_wait(acc_full + 8 * ac, aph ^ 1u, abort_flag)) { okw = false; break; }
-          const uint32_t at = scales + slot * kSlotBytes + (uint32_t)r0 * (4 * kNS);
-          if (kNS == 2) {
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(x0), "f"(y0) : "memory");
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + 64u * 8u), "f"(x1), "f"(y1) : "memory");
-          } else {
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x0) : "memory");
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 64u * 4u), "f"(x1) : "memory");
+          const uint32_t at = scales + ((slot + (uint32_t)k) & (kSlots - 1)) * kSlotBytes + (uint32_t)r0 * (4 * kNS);
+#pragma unroll
+          for (uint32_t j = 0; j < kLoads; ++j) {
+            if (kNS == 2) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + j * (8u * kRows)), "f"(v[j] * f0), "f"(v[j] * f1) : "memory");
+            else asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + j * (4u * kRows)), "f"(v[j] * f0) : "memory");
           }
+          if (kb + kChunk < kb_hi) fetch(m0, n0, kb + kChunk);
+          else if (more) fetch(next_m0, next_n0, kb_lo);
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(acc_full + 8 * ac);
-          if (++ac == kAccs) { ac = 0; aph ^= 1u; }
-          if (++slot == kSlots) slot = 0;
+          tell();
+          for (int j = 1; j < kChunk && kb + j < kb_hi; ++j) {
+            if (!ptx::warp_wait(acc_full + 8 * ac, aph ^ 1u, abort_flag)) { okw = false; break; }
+            tell();
+          }
         }
+        m0 = next_m0;
+        n0 = next_n0;
       }
       if (!okw && lane == 0 && p.error_flag) atomicCAS(p.error_flag, 0, (int)kErrWaitLoader);
     }
   } else {
     // ------------------------------------------------------------------ scaled sums -----
     // A part's 64 columns come in two loads; while one is added up the next is on its way, that of the next part or block too.
-    if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int quad = warp & 3, group = (warp - 4) >> 2;      // tensor-memory lanes this warp may read; which columns of each part
     const uint32_t release_at = PAIR ? ptx::map_to_cta(acc_empty, 0) : acc_empty;
     const uint32_t my_tmem = tmem_base + ((uint32_t)(quad * 32) << 16) + group * 64, my_scales = scales + (uint32_t)(quad * 32 + lane) * (4 * kNS);
@@ -381,7 +395,7 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     };
     auto advance = [&]() {
       if (++ac == kAccs) { ac = 0; aph ^= 1u; }
-      if (++slot == kSlots) slot = 0;
+      slot = (slot + 1) & (kSlots - 1);
     };
     int m0, n0;
     for (int i = 0; okw && item(i, m0, n0); ++i) {
@@ -563,11 +577,11 @@ size_t smem_of(int a_rows, int* stages) {
 
 // Tile and CTAs that share a tile's blocks: the least of a model's times, in us: rounds x (blocks x time of one + end of a tile) + launch
 // (+ exchange of partial sums).  A block of 128 takes longer with more rows of A, up to a whole tile.  The constants are fitted to 90
-// shapes (M and N 1 .. 8192, K 16 .. 8192), each timed with every tile and split that fits: the choice is 0.6 % above the fastest on
-// average, 20 % at worst (1594 x 1616 x 64: 256 x 256 on pairs 5.6 us, 128 x 64 4.7).
+// shapes (M and N 1 .. 8192, K 16 .. 8192), each timed with every tile and split that fits: the choice is 0.5 % above the fastest on
+// average, 9 % at worst (1024^3: 128 x 64 6.0 us, 256 x 128 on pairs 5.5).
 int pick(int M, int N, int KB, int sms, int* splits) {
   struct Tile { int m, n; double block, more, round, launch; };
-  static const Tile tiles[4] = {{128, 64, 0.16, 0.11, 0.75, 1.7}, {128, 128, 0.17, 0.20, 1.0, 1.8}, {256, 128, 0.30, 0.0, 1.1, 2.2}, {256, 256, 0.41, 0.0, 2.2, 1.9}};
+  static const Tile tiles[4] = {{128, 64, 0.16, 0.11, 0.75, 1.7}, {128, 128, 0.17, 0.20, 1.0, 1.8}, {256, 128, 0.27, 0.0, 1.1, 2.2}, {256, 256, 0.42, 0.0, 2.5, 2.0}};
   int stages;
   static const ClusterFit fit64 = cluster_fit(gemm_e4m3_kernel<64, false>, threads_of(64), smem_of<64, false>(kBM, &stages), sms);
   static const ClusterFit fit128 = cluster_fit(gemm_e4m3_kernel<128, false>, threads_of(128), smem_of<128, false>(kBM, &stages), sms);

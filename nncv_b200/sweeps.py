@@ -1,6 +1,6 @@
 """Kernel and network sweeps over the benchmark configs other than the headline one.
 
-    python -m nncv_b200.sweeps [gemm [SIZE]] [conv] [nets] [nets_f32 [BATCH]] [hbm] [mobilenet [BATCH]]
+    python -m nncv_b200.sweeps [gemm [SIZE]] [conv] [nets] [nets_f32 [BATCH]] [hbm] [linear8] [mobilenet [BATCH]]
 
   gemm : M=N=K in {512,1024,2048,4096}, fp16 in / fp32 accumulate (fp16 and fp32 C), optional fused
          bias + ReLU, and fp32 (config 1).
@@ -11,6 +11,8 @@
   hbm  : the memory-bound operators (depthwise conv + BN + hard-swish, activations, SE scaling, concat,
          2x upsampling, max-pool, global average pool) on MobileNetV3 / YOLOv5-sized maps: GB/s of
          algorithmic bytes (elements read + written) against the measured HBM copy bandwidth.
+  linear8 : a linear layer in 8 bits, as a block of a transformer has it (width 4096, bf16): norm with residual to e4m3, the
+         product, gated activation to e4m3, quantisation, for 1 to 4096 rows: GB/s and TFLOP/s.
   mobilenet : MobileNetV3-small fp16 @224 from a layer plan file (default: the plan the importer wrote from nncv's
          tests/Nets/MobileNetV3.mlir, kept under tests/golden/), seeded weights, batch 256 unless given.
 One JSON line per measurement; times are CUDA-event medians on the launching stream with an L2 flush
@@ -26,7 +28,7 @@ import numpy as np
 import torch
 
 from . import runtime as rt
-from ._lib import BF16, F16, F32, check, lib
+from ._lib import BF16, E4M3, F16, F32, check, lib
 
 PEAK_TF = 1644.0
 _flush = None
@@ -182,6 +184,35 @@ def hbm_ops():
     return out
 
 
+def linear8(width=4096):
+    st = torch.cuda.current_stream().cuda_stream
+    L = lib()
+    new = lambda *shape, dtype=torch.bfloat16: torch.empty(shape, device="cuda", dtype=dtype)
+    e4, blocks = torch.float8_e4m3fn, lambda k: -(-k // 128)
+
+    def rec(op, rows, nbytes, flops, fn):
+        ms = _time(fn, reps=9)
+        print(json.dumps({"sweep": "linear8", "op": op, "rows": rows, "us": round(ms * 1e3, 2), "gbs": round(nbytes / ms / 1e6, 1),
+                          "frac_of_hbm": round(nbytes / ms / 1e6 / PEAK_GBS, 3), "tflops": round(flops / ms / 1e9, 1)}), flush=True)
+
+    W = torch.randn((width, width), device="cuda") / width ** 0.5
+    Wq, Ws = new(width, width, dtype=e4), new(blocks(width), blocks(width), dtype=torch.float32)
+    rec("quantise fp32 weights, 128 x 128", width, 5 * width * width, 0,
+        lambda: check(L.nncv_b200_quantize_e4m3(_p(W), 0, F32, _p(Wq), _p(Ws), width, width, 128, st)))
+    gamma = torch.rand(width, device="cuda") + 0.5
+    for m in (1, 16, 128, 1024, 4096):
+        X, R, S, G = (torch.randn((m, width), device="cuda").bfloat16() for _ in range(4))
+        Q, Qs, C = new(m, width, dtype=e4), new(m, blocks(width), dtype=torch.float32), new(m, width)
+        scales = 4 * m * blocks(width)
+        rec("norm + residual to e4m3", m, 7 * m * width + scales + 4 * width, 0,
+            lambda: check(L.nncv_b200_rmsnorm(_p(X), 0, _p(R), _p(gamma), 1e-6, _p(S), _p(Q), E4M3, _p(Qs), BF16, m, width, st)))
+        rec("gated SiLU to e4m3", m, 5 * m * width + scales, 0,
+            lambda: check(L.nncv_b200_gated_activation(_p(X), _p(G), 0, _p(Q), E4M3, _p(Qs), BF16, m, width, 5, st)))
+        rec("quantise rows", m, 3 * m * width + scales, 0, lambda: check(L.nncv_b200_quantize_e4m3(_p(X), 0, BF16, _p(Q), _p(Qs), m, width, 1, st)))
+        rec("matmul to bf16", m, 3 * m * width + width * width, 2.0 * m * width * width,
+            lambda: check(L.nncv_b200_matmul_e4m3(_p(Q), _p(Qs), _p(Wq), _p(Ws), _p(C), m, width, width, BF16, None, 0, st)))
+
+
 def mobilenet(batch=256, plan_path=None):
     import os
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -225,6 +256,8 @@ if __name__ == "__main__":
         gemm(sizes or (512, 1024, 2048, 4096))
     if "hbm" in which:
         hbm_ops()
+    if "linear8" in which:
+        linear8()
     if "conv" in which:
         conv()
     if "conv256" in which:
