@@ -355,14 +355,15 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
  * leaves the rest of its block as it is.  Scales of an [M,K] matrix: [M, ceil(K/128)] (activations: one for 128 columns of a row) or
  * [ceil(M/128), ceil(K/128)] (weights: one for 128 x 128), row-major; the last block of a row may be shorter.
  * Rows of x, gate and up may lie further apart than K (ldx, ld: elements from row to row, 0 = K); all else is dense.  M = 0 is
- * a call that does nothing.  All pointers belong to the current device.  Everything computes in fp32; an fp16 result beyond its range becomes +-65504.  Any K and any
- * address of an element are allowed; K a multiple of 8 with everything on 16-byte boundaries is read 16 bytes at a time.
+ * a call that does nothing.  All pointers belong to the current device.  Everything computes in fp32; an fp16 result beyond its
+ * range becomes +-65504.  The norm, the activation and the quantisation take any K and any address of an element; with K a multiple
+ * of 8 and everything on 16-byte boundaries they read 16 bytes at a time.
  *
  * Root-mean-square norm of x, or of h = x + residual: out = h / sqrt(mean(h^2) + eps) * weight.
  *   x [M,K] of dtype; residual [M,K] of dtype or NULL; weight fp32 [K] or NULL (= 1)
  *   sum: NULL, or [M,K] of dtype that receives h (the norm is taken of h before this rounding); may be residual, or x where ldx is K
  *   out: [M,K] of out_dtype, which is dtype or NNCV_B200_E4M3; scale: fp32 [M, ceil(K/128)] with E4M3, else NULL
- * out may be x (where ldx is K) or residual, if it has their type. */
+ * out may be x (where ldx is K) or residual, if it has their type.  A row whose squares' sum passes fp32's range gives zeros. */
 int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const void* weight, float eps, void* sum, void* out, int out_dtype,
                       float* scale, int dtype, int M, int K, void* stream);
 /* out = activation(gate) * up, or activation(gate) where up is NULL.  gate and up [M,K] of dtype, rows ld apart: the halves of one
@@ -372,10 +373,10 @@ int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, v
                                int act, void* stream);
 /* x [M,K] of dtype to e4m3 q [M,K] with a scale for block_rows x 128 values, block_rows 1 or 128. */
 int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, float* scale, int M, int K, int block_rows, void* stream);
-/* C[M,N] = A * B^T (+ bias[N]) (+ ReLU): A [M,K] e4m3 with scales [M, ceil(K/128)], B [N,K] e4m3 (as a fully connected layer stores
- * its weights) with scales [ceil(N/128), ceil(K/128)]; C of c_dtype F32, F16 or BF16.  K a multiple of 16, A and B on 16-byte boundaries, C on any
- * element's.  fp32 sums; a block's sum is scaled before it is added to the others.  No scratch: calls on several streams, and captured
- * calls, share nothing. */
+/* C[M,N] = A * B^T (+ bias[N]) (+ ReLU): A [M,K] e4m3 with scales [M, ceil(K/128)], B [N,K] e4m3 (as a fully connected layer
+ * stores its weights) with scales [ceil(N/128), ceil(K/128)]; C of c_dtype F32, F16 or BF16.  K a multiple of 16, A and B on 16-byte
+ * boundaries, C on any element's.  fp32 sums; a block's sum is scaled before it is added to the others.  C must not overlap an operand.
+ * No scratch: calls on several streams, and captured calls, share nothing. */
 int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, const float* scale_b, void* C, int M, int N, int K, int c_dtype,
                           const float* bias, int relu, void* stream);
 

@@ -9,6 +9,16 @@
 // Roles: warp 0 copies, warp 1 issues the MMAs, warps 2 and 3 bring the products of the scales, the others add up and store.
 // Rows and columns behind M and N read as zero and are not stored.  Every wait is bounded and abortable; one that runs out sets
 // the device status word.
+//
+// What bounds it.  Large: the power limit.  A block of a 256 x 256 tile on a CTA pair is 512 clocks of MMAs; copies and MMAs alone take
+// 540, with the sums taken out and scaled 640, with the result's stores 708 on average; the clock falls from 1.97 to 1.3 GHz.
+// 8192 x 8192 x 4096 to bf16: 227 us in a burst (2420 TFLOP/s), 270 back to back; MMAs, copies and hand-overs alone 171 and 216, the
+// vendor library's product with one scale a matrix 186 and 225.  The epilogue warps of an SM quarter need 256 clocks of
+// multiply-adds and 180 of tensor-memory loads a block, and the two do not overlap; sixteen epilogue warps instead of eight were 7 %
+// slower, one release of both parts 2 %, one wait a part 3 %, halves of tiles in the last round no faster.
+// Middle sizes: what an SM takes in from L2, about 56 bytes a clock (a block of 128 x 128 is 32 KB: 600 clocks where its MMAs take 256).
+// Few rows: reading B (4.4 TB/s of 6.5 at 16 x 8192 x 8192), and for one small layer what is fixed: of the 6.4 us of 1 x 4096 x 4096
+// 1.9 pass until the first block is here, 2 while B comes, 1.9 while the CTAs of a cluster meet and add up.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -48,7 +58,7 @@ struct GeParams {
   int splits_log;             // (as a power of two) CTAs of a cluster that share a tile's blocks; then every cluster has one tile
 };
 
-__device__ __forceinline__ void stage_bias_relu(const GeParams& p, int n, float (&v)[8]) {
+__device__ __forceinline__ void bias_relu(const GeParams& p, int n, float (&v)[8]) {
   if (p.bias) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -62,6 +72,8 @@ __device__ __forceinline__ void stage_bias_relu(const GeParams& p, int n, float 
 
 // 32 rows (a lane each) of 64 columns of a warp's sums from (row, col) on: bias, ReLU, and through the warp's staging buffers out
 // of the SM.  TYPE: DType of the result; PLAIN: neither bias nor ReLU.
+// (900 clocks a slab: 200 until it is known that the buffer is free, 350 to convert, 250 for the fence between stores and copy.  With rows
+// read back and stored in 16-byte pieces 1400 to 2000, with each lane storing its own row's pieces 3500.)
 template <int TYPE, bool PLAIN>
 __device__ __forceinline__ void store_slab(const GeParams& p, const CUtensorMap* tm_c, uint32_t stage, uint32_t& turn, int row, int col, int lane,
                                            const unsigned long long (&sum)[32]) {
@@ -71,7 +83,7 @@ __device__ __forceinline__ void store_slab(const GeParams& p, const CUtensorMap*
 #pragma unroll
   for (int c = 0; c < 64; c += kSlab) {
     if (col + c >= p.N) break;
-    const uint32_t buf = stage + turn * 4096u, at = buf + (uint32_t)lane * 128u;
+    const uint32_t buf = stage + turn * epi::kBufBytes, at = buf + (uint32_t)lane * 128u;
     if (lane == 0) ptx::bulk_wait_read<kBufs - 1>();   // the copy that last read this buffer is done
     __syncwarp();
 #pragma unroll
@@ -79,7 +91,7 @@ __device__ __forceinline__ void store_slab(const GeParams& p, const CUtensorMap*
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) epi::unpk(sum[c / 2 + h * 4 + i], v[2 * i], v[2 * i + 1]);
-      if (!PLAIN) stage_bias_relu(p, col + c + h * 8, v);
+      if (!PLAIN) bias_relu(p, col + c + h * 8, v);
       if (kF) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -128,9 +140,9 @@ __device__ __forceinline__ void add_chunk(const uint32_t (&v)[32], unsigned long
   for (int i = 0; i < 16; ++i) sum[AT / 2 + i] = epi::fma2(epi::pk(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), s2, sum[AT / 2 + i]);
 }
 
-// Tiles of 128 x 64 or 128 x 128 (one CTA, or a cluster that shares the tile's blocks), or of 256 x 256 on a CTA pair: there an
-// accumulator has two parts of 128 columns, which are given back one after the other, so that the MMAs of the next block but one
-// start when half of this one has been read.
+// Tiles of 128 x 64 or 128 x 128 (one CTA, or a cluster that shares the tile's blocks), or of 256 x 128 or 256 x 256 on a CTA pair.  Of
+// the last, an accumulator has two parts of 128 columns, which are given back one after the other, so that the MMAs of the next
+// block but one start when half of this one has been read (in one part: 239 us instead of 234 at 8192 x 8192 x 4096).
 template <int BN, bool PAIR>
 __global__ void __launch_bounds__(threads_of(BN), 1)
 gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_c,
