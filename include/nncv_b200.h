@@ -358,6 +358,8 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
  * a call that does nothing.  All pointers belong to the current device.  Everything computes in fp32; an fp16 result beyond its
  * range becomes +-65504.  The norm, the activation and the quantisation take any K and any address of an element; with K a multiple
  * of 8 and everything on 16-byte boundaries they read 16 bytes at a time.
+ * The library's first call on a device sets it up and cannot be captured into a graph (nncv_b200_device_status() is one that will do);
+ * after it any call of these four can.
  *
  * Root-mean-square norm of x, or of h = x + residual: out = h / sqrt(mean(h^2) + eps) * weight.
  *   x [M,K] of dtype; residual [M,K] of dtype or NULL; weight fp32 [K] or NULL (= 1)

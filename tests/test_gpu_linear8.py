@@ -479,3 +479,42 @@ def test_two_captured_blocks_replayed_with_new_inputs():
         status()
         for b in blocks:
             b.verify()
+
+
+FIRST_CALLS_IN_A_CAPTURE = """
+import torch
+from nncv_b200._lib import F32, check, lib
+L = lib()
+x = torch.randn(256, 512, device="cuda")
+e4, p = torch.float8_e4m3fn, lambda t: t.data_ptr()
+q, s = torch.empty(256, 512, device="cuda", dtype=e4), torch.empty(256, 4, device="cuda")
+wq, ws = torch.empty(256, 512, device="cuda", dtype=e4), torch.empty(2, 4, device="cuda")
+c, y = torch.empty(256, 256, device="cuda"), torch.empty_like(x)
+check(L.nncv_b200_device_status())   # sets the library up on this device
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    check(L.nncv_b200_quantize_e4m3(p(x), 0, F32, p(q), p(s), 256, 512, 1, st))
+    check(L.nncv_b200_quantize_e4m3(p(x), 0, F32, p(wq), p(ws), 256, 512, 128, st))
+    check(L.nncv_b200_matmul_e4m3(p(q), p(s), p(wq), p(ws), p(c), 256, 256, 512, F32, None, 0, st))
+    check(L.nncv_b200_rmsnorm(p(x), 0, None, None, 1e-6, None, p(y), F32, None, F32, 256, 512, st))
+    check(L.nncv_b200_gated_activation(p(y), None, 0, p(y), F32, None, F32, 256, 512, 0, st))
+x.mul_(2.0)
+g.replay()
+torch.cuda.synchronize()
+# two roundings to e4m3 of half a step of 2^-3 at most, independent: the norm of the error is well below their sum
+ref = x.double() @ x.double().T
+assert ((c.double() - ref).norm() / ref.norm()).item() <= 2 * 2.0 ** -4
+assert (y.double() - x.double() / torch.sqrt(x.double().square().mean(1, keepdim=True) + 1e-6)).abs().max().item() <= 6 * 48 * 2.0 ** -24
+check(L.nncv_b200_device_status())
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_in_a_capture():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS_IN_A_CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout[-500:] + done.stderr[-2000:]
