@@ -3087,8 +3087,9 @@ int nncv_b200_bn_fold(const void* gamma, const void* beta, const void* mean, con
 // ---- a linear layer in 8 bits -------------------------------------------------------------
 static bool on_boundary(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 static bool of_type(const void* p, int dtype) { return on_boundary(p, dtype_size((DType)dtype)); }
-// blocks of 128 columns are counted in 31 bits (their values alone would fill more than 250 GB)
-static bool too_many_blocks(int M, int K) { return (long long)M * (((long long)K + 127) / 128) > 0x7fffff00LL; }
+// columns, and blocks of 128 of them, are counted in 31 bits with room for a last step beyond the end
+constexpr int kMostColumns = 1 << 30;
+static bool too_large(int M, int K) { return K > kMostColumns || (long long)M * (((long long)K + 127) / 128) > 0x7fffff00LL; }
 // out_dtype is dtype or E4M3, and scales go with E4M3 alone
 static int check_out(const char* what, int out_dtype, int dtype, const void* out, const float* scale) {
   if (out_dtype != dtype && out_dtype != NNCV_B200_E4M3) return fail(NNCV_B200_EINVAL, "%s: out_dtype must be dtype or E4M3", what);
@@ -3104,7 +3105,7 @@ int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const 
   if (!x || !out || M < 0 || K <= 0 || dtype < 0 || dtype > 2 || !(eps >= 0.0f)) return fail(NNCV_B200_EINVAL, "rmsnorm: bad argument");
   if (ldx == 0) ldx = K;
   if (ldx < K) return fail(NNCV_B200_EINVAL, "rmsnorm: ldx is less than K");
-  if (too_many_blocks(M, K)) return fail(NNCV_B200_EINVAL, "rmsnorm: more than 2^31 blocks of 128");
+  if (too_large(M, K)) return fail(NNCV_B200_EINVAL, "rmsnorm: more than 2^30 columns or 2^31 blocks of 128");
   if (!of_type(x, dtype) || !of_type(residual, dtype) || !of_type(sum, dtype) || !on_boundary(weight, 4))
     return fail(NNCV_B200_EINVAL, "rmsnorm: a pointer is not on its type's boundary");
   if ((rc = check_out("rmsnorm", out_dtype, dtype, out, scale))) return rc;
@@ -3125,7 +3126,7 @@ int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, v
   if (!gate || !out || M < 0 || K <= 0 || dtype < 0 || dtype > 2 || act < 0 || act > 5) return fail(NNCV_B200_EINVAL, "gated_activation: bad argument");
   if (ld == 0) ld = K;
   if (ld < K) return fail(NNCV_B200_EINVAL, "gated_activation: ld is less than K");
-  if (too_many_blocks(M, K)) return fail(NNCV_B200_EINVAL, "gated_activation: more than 2^31 blocks of 128");
+  if (too_large(M, K)) return fail(NNCV_B200_EINVAL, "gated_activation: more than 2^30 columns or 2^31 blocks of 128");
   if (!of_type(gate, dtype) || !of_type(up, dtype)) return fail(NNCV_B200_EINVAL, "gated_activation: a pointer is not on its type's boundary");
   if ((rc = check_out("gated_activation", out_dtype, dtype, out, scale))) return rc;
   if ((out == gate || out == up) && (ld != K || out_dtype == NNCV_B200_E4M3))
@@ -3145,7 +3146,7 @@ int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, fl
   if (block_rows != 1 && block_rows != 128) return fail(NNCV_B200_EINVAL, "quantize_e4m3: block_rows must be 1 or 128");
   if (ldx == 0) ldx = K;
   if (ldx < K) return fail(NNCV_B200_EINVAL, "quantize_e4m3: ldx is less than K");
-  if (too_many_blocks(M, K)) return fail(NNCV_B200_EINVAL, "quantize_e4m3: more than 2^31 blocks of 128");
+  if (too_large(M, K)) return fail(NNCV_B200_EINVAL, "quantize_e4m3: more than 2^30 columns or 2^31 blocks of 128");
   if (!of_type(x, dtype) || !on_boundary(scale, 4)) return fail(NNCV_B200_EINVAL, "quantize_e4m3: a pointer is not on its type's boundary");
   if (q == x) return fail(NNCV_B200_EINVAL, "quantize_e4m3: q needs memory of its own");
   if ((rc = device_init()) || M == 0) return rc ? rc : ok();
@@ -3166,7 +3167,8 @@ int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, co
   if (!A || !scale_a || !B || !scale_b || !C || M < 0 || N <= 0 || K <= 0) return fail(NNCV_B200_EINVAL, "matmul_e4m3: bad argument");
   if (c_dtype < 0 || c_dtype > 2) return fail(NNCV_B200_EINVAL, "matmul_e4m3: c_dtype must be F32, F16 or BF16");
   if (K % 16 != 0) return fail(NNCV_B200_EINVAL, "matmul_e4m3: K must be a multiple of 16");
-  if (((long long)M + 127) / 128 * (((long long)N + 63) / 64) > 0x3fffffffLL) return fail(NNCV_B200_EINVAL, "matmul_e4m3: more than 2^30 tiles of 128 x 64");
+  if (M > kMostColumns || N > kMostColumns || K > kMostColumns || ((long long)M + 127) / 128 * (((long long)N + 63) / 64) > 0x3fffffffLL)
+    return fail(NNCV_B200_EINVAL, "matmul_e4m3: a side longer than 2^30, or more than 2^30 tiles of 128 x 64");
   if (!on_boundary(A, 16) || !on_boundary(B, 16)) return fail(NNCV_B200_EINVAL, "matmul_e4m3: A and B must lie on 16-byte boundaries");
   if (!of_type(C, c_dtype) || !on_boundary(scale_a, 4) || !on_boundary(scale_b, 4) || !on_boundary(bias, 4))
     return fail(NNCV_B200_EINVAL, "matmul_e4m3: a pointer is not on its type's boundary");

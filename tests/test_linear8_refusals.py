@@ -29,7 +29,7 @@ def matmul(a=P, sa=2 * P, b=3 * P, sb=4 * P, c=5 * P, m=4, n=8, k=256, cdt=BF16,
 
 @pytest.mark.parametrize("bad", [
     dict(x=None), dict(out=None), dict(m=-1), dict(k=0), dict(k=-8), dict(dt=3), dict(dt=-1), dict(eps=-1e-6), dict(eps=float("nan")),
-    dict(ldx=255), dict(ldx=-1), dict(m=1 << 30, k=1 << 10), dict(out_dt=F16, scale=None), dict(out_dt=4), dict(scale=None), dict(out_dt=BF16), dict(x=P + 1), dict(res=P + 1),
+    dict(ldx=255), dict(ldx=-1), dict(m=1 << 30, k=1 << 10), dict(m=1, k=(1 << 30) + 16), dict(out_dt=F16, scale=None), dict(out_dt=4), dict(scale=None), dict(out_dt=BF16), dict(x=P + 1), dict(res=P + 1),
     dict(sum_=P + 1), dict(w=P + 2), dict(scale=P + 2), dict(dt=F32, x=P + 2), dict(out_dt=BF16, scale=None, out=P + 1),
     dict(sum_=P, ldx=264), dict(out=4 * P), dict(out=P), dict(out=2 * P), dict(out=P, ldx=264, out_dt=BF16, scale=None)])
 def test_rmsnorm_refuses(bad):
@@ -37,7 +37,7 @@ def test_rmsnorm_refuses(bad):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(gate=None), dict(out=None), dict(m=-1), dict(k=0), dict(dt=3), dict(act=6), dict(act=-1), dict(ld=255), dict(m=1 << 30, k=1 << 10), dict(out_dt=F32, scale=None),
+    dict(gate=None), dict(out=None), dict(m=-1), dict(k=0), dict(dt=3), dict(act=6), dict(act=-1), dict(ld=255), dict(m=1 << 30, k=1 << 10), dict(m=1, k=(1 << 30) + 16), dict(out_dt=F32, scale=None),
     dict(scale=None), dict(out_dt=BF16), dict(gate=P + 1), dict(up=P + 1), dict(scale=P + 1), dict(out=P), dict(out=2 * P),
     dict(out=P, out_dt=BF16, scale=None, ld=512)])
 def test_gated_activation_refuses(bad):
@@ -45,7 +45,7 @@ def test_gated_activation_refuses(bad):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(x=None), dict(q=None), dict(scale=None), dict(m=-1), dict(k=0), dict(dt=3), dict(ldx=100), dict(m=1 << 30, k=1 << 10), dict(m=1 << 30, k=1 << 10, rows=128), dict(rows=0), dict(rows=64), dict(rows=256),
+    dict(x=None), dict(q=None), dict(scale=None), dict(m=-1), dict(k=0), dict(dt=3), dict(ldx=100), dict(m=1 << 30, k=1 << 10), dict(m=1, k=(1 << 30) + 16), dict(m=1 << 30, k=1 << 10, rows=128), dict(rows=0), dict(rows=64), dict(rows=256),
     dict(x=P + 1), dict(scale=P + 2), dict(q=P)])
 def test_quantize_refuses(bad):
     assert quantize(**bad) == EINVAL and b"quantize_e4m3" in lib().nncv_b200_last_error()
@@ -53,7 +53,7 @@ def test_quantize_refuses(bad):
 
 @pytest.mark.parametrize("bad", [
     dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(c=None), dict(m=-1), dict(n=0), dict(k=0), dict(k=8), dict(k=250), dict(cdt=3),
-    dict(cdt=-1), dict(a=P + 8), dict(b=P + 1), dict(c=P + 1), dict(cdt=F32, c=P + 2), dict(sa=P + 2), dict(sb=P + 1), dict(bias=P + 2), dict(m=1 << 30, n=1 << 20)])
+    dict(cdt=-1), dict(a=P + 8), dict(b=P + 1), dict(c=P + 1), dict(cdt=F32, c=P + 2), dict(sa=P + 2), dict(sb=P + 1), dict(bias=P + 2), dict(m=1 << 30, n=1 << 20), dict(m=(1 << 30) + 1), dict(n=(1 << 30) + 1), dict(k=(1 << 30) + 16)])
 def test_matmul_refuses(bad):
     assert matmul(**bad) == EINVAL and b"matmul_e4m3" in lib().nncv_b200_last_error()
 
