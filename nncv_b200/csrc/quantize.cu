@@ -100,7 +100,12 @@ __device__ __forceinline__ void infinite_to_nan(float (&v)[kV]) {   // the conve
 #pragma unroll
   for (int e = 0; e < kV; ++e) v[e] = fabsf(v[e]) < INFINITY ? v[e] : __int_as_float(0x7fffffff);
 }
-__device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax, kLeast) * (1.0f / kTop); }
+// max / 448 as the division rounds it: the product with 1 / 448, corrected by its remainder (as for the quotients below; the same for all 2^23
+// mantissas).
+__device__ __forceinline__ float block_scale(float amax) {
+  const float a = fmaxf(amax, kLeast), s = a * (1.0f / kTop);
+  return fmaf(fmaf(s, -kTop, a), 1.0f / kTop, s);
+}
 __device__ __forceinline__ float reciprocal(float s) {   // a step of fp32 off at most where 1 / s is a normal number
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
@@ -111,16 +116,35 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// Minus y / s for two values of a block.  The product with the approximate 1 / s is at most 2.5 steps of fp32 off; its remainder, by a fused
+// multiply-add, times 1 / s corrects it to 2^-21 of a step before the last rounding (after P. Markstein, Computation of elementary functions
+// on the IBM RISC System/6000, 1990).  So a quotient half way between two e4m3 values comes out as that and goes to the even one, where the
+// product alone sent some to the other.  The sign is turned twice, so that a zero keeps its own.  8192 x 2048 bf16
+// in rows takes 9.4 us, with the product alone 9.1; gated 2048 x 8192 13.9 for 13.7; 4096 x 4096 bf16 in blocks 12.3 for 11.6.
+struct Divisor {
+  unsigned long long s, minus_inv;
+  __device__ __forceinline__ explicit Divisor(float by) : s(epi::pk(by, by)) {
+    const float r = -reciprocal(by);
+    minus_inv = epi::pk(r, r);
+  }
+  __device__ __forceinline__ void divide(float a, float b, float& qa, float& qb) const {
+    const unsigned long long y = epi::pk(a, b), q = epi::mul2(y, minus_inv);
+    epi::unpk(epi::fma2(epi::fma2(q, s, y), minus_inv, q), qa, qb);
+  }
+};
 template <bool VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* row, int col0, int t, int K, const float (&v)[kV], float inv) {
+__device__ __forceinline__ void store_e4m3(uint8_t* row, int col0, int t, int K, const float (&v)[kV], const Divisor& by) {
 #pragma unroll
   for (int i = 0; i < kV / kPiece; ++i) {
     const int col = col0 + piece_col(i, t);
     uint32_t h[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float* q = v + i * kPiece + 4 * j;
-      h[j] = e4m3x2(q[0] * inv, q[1] * inv) | e4m3x2(q[2] * inv, q[3] * inv) << 16;
+      const float* y = v + i * kPiece + 4 * j;
+      float q[4];
+      by.divide(y[0], y[1], q[0], q[1]);
+      by.divide(y[2], y[3], q[2], q[3]);
+      h[j] = (e4m3x2(q[0], q[1]) | e4m3x2(q[2], q[3]) << 16) ^ 0x80808080u;
     }
     if (VEC) {
       if (col < K) *reinterpret_cast<uint2*>(row + col) = make_uint2(h[0], h[1]);
@@ -142,7 +166,7 @@ __device__ __forceinline__ void put_block(uint8_t* row, float* scale, int col0, 
     infinite_to_nan(v);
   }
   const float s = block_scale(amax);
-  store_e4m3<VEC>(row, col0, t, K, v, reciprocal(s));
+  store_e4m3<VEC>(row, col0, t, K, v, Divisor(s));
   if (t == 0 && col0 < K) *scale = s;
 }
 
@@ -348,12 +372,13 @@ __global__ void __launch_bounds__(kBlockThreads) quantize_block_kernel(const T* 
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kBlockThreads / 32; ++i) amax = fmaxf(amax, s_part[i]);
-  const float s = block_scale(amax), inv = reciprocal(s);
+  const float s = block_scale(amax);
+  const Divisor by(s);
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
 #pragma unroll
   for (int i = 0; i < kBlockIter; ++i) {
     const int row = r0 + i * kBlockRows;
-    if (row < M) store_e4m3<VEC>(q + (long long)row * K, col0, t, K, v[i], inv);
+    if (row < M) store_e4m3<VEC>(q + (long long)row * K, col0, t, K, v[i], by);
   }
 }
 

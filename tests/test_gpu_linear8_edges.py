@@ -1,0 +1,139 @@
+"""The 8-bit linear layer where a definition is easily missed: quotients at ties, gates far below zero, infinities, weights far from one,
+empty tensors, calls of several sizes in one graph."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+import linear8_ref as R  # noqa: E402
+from nncv_b200._lib import BF16, E4M3, F16, F32, check, lib  # noqa: E402
+from test_gpu_linear8 import ACT, DT, gen, guarded, p, run_gated, run_matmul, run_norm, status, stream  # noqa: E402
+
+U = R.U
+INF, NAN = float("inf"), float("nan")
+
+
+# ---------------------------------------------------------------------------------------------------------------- e4m3 of a quotient
+def quotients(x, rows):
+    """q and scales of finite fp32 values as the definition has them, each operation in fp32 and correctly rounded (on the CPU)."""
+    x = x.float().cpu()
+    m, k = x.shape
+    mb, kb = -(-m // rows), R.blocks(k)
+    pad = torch.zeros((mb * rows, kb * 128))
+    pad[:m, :k] = x
+    amax = pad.view(mb, rows, kb, 128).abs().amax(dim=(1, 3)).clamp_min(2.0 ** -100)
+    s = amax / torch.tensor(448.0)
+    return (x / s.repeat_interleave(rows, 0)[:m].repeat_interleave(128, 1)[:, :k]).clamp(-448, 448).to(torch.float8_e4m3fn), s
+
+
+def run_quantize(x, dt, rows):
+    m, k = x.shape
+    q, free = guarded(m, k, torch.float8_e4m3fn)
+    s, free_s = guarded(-(-m // rows), R.blocks(k), torch.float32)
+    check(lib().nncv_b200_quantize_e4m3(p(x), x.stride(0), dt, p(q), p(s), m, k, rows, stream()))
+    status()
+    free()
+    free_s()
+    return q, s
+
+
+def at_ties(m, k, seed):
+    """Values that lie half way between two e4m3 values times the scale of their block.  The scale has 15 bits, so that its products with 448
+    and with a midpoint (5 bits) are exact in fp32."""
+    g = torch.Generator().manual_seed(seed)
+    s = (torch.randint(2 ** 14, 2 ** 15, (m, R.blocks(k)), generator=g) | 1).float() * 2.0 ** -20
+    e = torch.randint(0, 14, (m, k), generator=g) - 6
+    half = (torch.randint(8, 16, (m, k), generator=g).float() + 0.5) / 8 * torch.exp2(e.float())
+    half = half.clamp_max(432.0) * (torch.randint(0, 2, (m, k), generator=g) * 2 - 1)
+    half[:, ::128] = 448.0
+    return half * s.repeat_interleave(128, 1)[:, :k]
+
+
+@pytest.mark.parametrize("m,k", [(300, 1024), (7, 1000), (64, 77)])
+def test_quantize_rows_at_ties(m, k):
+    x = at_ties(m, k, m + k)
+    want, s = quotients(x, 1)
+    q, got_s = run_quantize(x.cuda(), F32, 1)
+    assert torch.equal(got_s.cpu(), s)
+    assert R.exactly(q, want), (q.cpu().view(torch.uint8) != want.view(torch.uint8)).float().mean().item()
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("m,k,size", [(600, 2048, 1.0), (129, 1000, 1e-3), (600, 2048, 30.0)])
+def test_quantize_is_the_quotient(dt, rows, m, k, size):
+    x = (torch.randn((m, k), generator=gen(m, k, dt, rows), device="cuda") * size).to(DT[dt])
+    want, s = quotients(x, rows)
+    q, got_s = run_quantize(x, dt, rows)
+    assert torch.equal(got_s.cpu(), s)
+    assert R.exactly(q, want), (q.cpu().view(torch.uint8) != want.view(torch.uint8)).float().mean().item()
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("size", [3e38, 1e30, 1e-20, 1e-28, 1e-30, 3e-31, 1e-35, 1e-40])
+def test_quantize_is_the_quotient_at_both_ends_of_fp32(rows, size):
+    x = torch.rand((256, 512), generator=gen(rows), device="cuda").mul_(2).sub_(1).mul_(size)
+    want, s = quotients(x, rows)
+    q, got_s = run_quantize(x, F32, rows)
+    assert torch.equal(got_s.cpu(), s) and R.exactly(q, want)
+
+
+def test_scale_of_every_mantissa():
+    """Blocks of one value: all 2^23 mantissas, at three sizes."""
+    for size in (1.0, 1e-20, 1e20):
+        x = (torch.arange(2 ** 23, dtype=torch.int32) + 0x3F800000).view(torch.float32).view(-1, 1) * size
+        q, s = run_quantize(x.cuda(), F32, 1)
+        assert torch.equal(s.cpu(), x / torch.tensor(448.0)) and (q.float() == 448).all()
+
+
+@pytest.mark.parametrize("with_up", [True, False])
+def test_gated_to_e4m3_is_the_quotient(with_up):
+    """Without an activation the product is one rounding, so that every bit is known."""
+    g = gen(71, with_up)
+    gate, up = (torch.randn((300, 1024), generator=g, device="cuda").bfloat16() for _ in range(2))
+    out, s = run_gated(gate, up if with_up else None, "none", BF16, True)
+    want, want_s = quotients(gate.float() * up.float() if with_up else gate.float(), 1)
+    assert torch.equal(s.cpu(), want_s) and R.exactly(out, want)
+
+
+# ---------------------------------------------------------------------------------------------------------------- several sizes in one graph
+def test_products_of_several_heights_in_one_graph():
+    """Fewer rows take less shared memory: neither a later node of the graph nor a call between its capture and its replay takes
+    away what an earlier node needs."""
+    g = gen(95)
+    b, sb = R.operand(g, 512, 1024, 128)
+    ops = [R.operand(g, m, 1024, 1) for m in (128, 100, 64, 40, 17, 8, 1)]
+    outs = [torch.empty((a.shape[0], 512), device="cuda") for a, _ in ops]
+
+    def all_of(which):
+        for i in which:
+            (a, sa), c = ops[i], outs[i]
+            check(lib().nncv_b200_matmul_e4m3(p(a), p(sa), p(b), p(sb), p(c), a.shape[0], 512, 1024, F32, None, 0, stream()))
+    all_of(range(len(ops)))
+    status()
+    want = [c.clone() for c in outs]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        all_of(range(len(ops)))
+    for last in (len(ops) - 1, 0):
+        all_of([last])
+        status()
+        for c in outs:
+            c.fill_(NAN)
+        gr.replay()
+        status()
+        assert all(torch.equal(c, w) for c, w in zip(outs, want))
+
+
+# ---------------------------------------------------------------------------------------------------------------- the same bits
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_every_call_gives_the_same_bits(e4m3):
+    g = gen(96)
+    t = torch.randn((512, 8192), generator=g, device="cuda").bfloat16()
+    w = torch.randn(4096, generator=g, device="cuda")
+    first = None
+    for _ in range(4):
+        got = [o for o in run_gated(t[:, :4096], t[:, 4096:], "silu", BF16, e4m3) + run_norm(t[:, :4096], t[:, 4096:].contiguous(), w, 1e-6, BF16, e4m3, True)
+               if o is not None]
+        first = first or got
+        assert all(R.exactly(a, b) for a, b in zip(got, first))
