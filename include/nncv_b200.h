@@ -351,9 +351,10 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
 /* ---- a linear layer in 8-bit floating point (device pointers; `stream` is a cudaStream_t; no synchronisation) ----
  * No counterpart in the reference, whose matmuls are 16-bit and fp32.  Values are e4m3 (one byte: 4 exponent bits, 3 mantissa
  * bits, largest 448, no infinity) with one fp32 scale for each block of 128: value = byte * scale.  A block of values y is written
- * with scale = max(largest finite |y|, 2^-100) / 448 and y / scale rounded to nearest; an infinity or a NaN becomes NaN and
- * leaves the rest of its block as it is.  Scales of an [M,K] matrix: [M, ceil(K/128)] (activations: one for 128 columns of a row) or
- * [ceil(M/128), ceil(K/128)] (weights: one for 128 x 128), row-major; the last block of a row may be shorter.
+ * with scale = max(largest finite |y|, 2^-100) * (1/448 in fp32) and the fp32 quotient y / scale rounded to the nearest value, to the
+ * even one at a tie; an infinity or a NaN becomes NaN and leaves the rest of its block as it is.  Scales of an [M,K] matrix:
+ * [M, ceil(K/128)] (activations: one for 128 columns of a row) or [ceil(M/128), ceil(K/128)] (weights: one for 128 x 128), row-major;
+ * the last block of a row may be shorter.
  * Rows of x, gate and up may lie further apart than K (ldx, ld: elements from row to row, 0 = K); all else is dense.  M = 0 is
  * a call that does nothing; no row, and no side of a product, is longer than 2^30.  All pointers belong to the current device.
  * Everything computes in fp32; an fp16 result beyond its range becomes +-65504.  The norm, the activation and the quantisation take

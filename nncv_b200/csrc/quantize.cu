@@ -1,7 +1,7 @@
 // What makes the operands of the 8-bit matrix product: root-mean-square norm with the residual's addition, gated
 // activations and plain quantisation, each with an e4m3 result that carries a scale for every block of 128 values.
 //
-// A block of values y:  s = max(largest finite |y|, 2^-100) / 448,  q = y / s rounded to e4m3 (448 is its largest value).
+// A block of values y:  s = max(largest finite |y|, 2^-100) * (1 / 448),  q = y / s rounded to e4m3 (448 is its largest value).
 // The least scale keeps 1 / s finite for a block of zeros.  What is not finite becomes NaN -- e4m3 has no infinity -- and leaves
 // the other values of its block as they are.
 //
@@ -100,12 +100,8 @@ __device__ __forceinline__ void infinite_to_nan(float (&v)[kV]) {   // the conve
 #pragma unroll
   for (int e = 0; e < kV; ++e) v[e] = fabsf(v[e]) < INFINITY ? v[e] : __int_as_float(0x7fffffff);
 }
-// max / 448 as the division rounds it: the product with 1 / 448, corrected by its remainder (as for the quotients below; the same for all 2^23
-// mantissas).
-__device__ __forceinline__ float block_scale(float amax) {
-  const float a = fmaxf(amax, kLeast), s = a * (1.0f / kTop);
-  return fmaf(fmaf(s, -kTop, a), 1.0f / kTop, s);
-}
+// Times 1 / 448 as fp32 has it: a step off the quotient for some, which the values' own quotient by it makes up for.
+__device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax, kLeast) * (1.0f / kTop); }
 __device__ __forceinline__ float reciprocal(float s) {   // a step of fp32 off at most where 1 / s is a normal number
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
