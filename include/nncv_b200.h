@@ -371,7 +371,8 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
 int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const void* weight, float eps, void* sum, void* out, int out_dtype,
                       float* scale, int dtype, int M, int K, void* stream);
 /* out = activation(gate) * up, or activation(gate) where up is NULL.  gate and up [M,K] of dtype, rows ld apart: the halves of one
- * [M,2K] tensor are gate = t, up = t + K, ld = 2K.  act: NNCV_B200_ACT_*.  out and scale as above; out may be gate or up where ld is K and the
+ * [M,2K] tensor are gate = t, up = t + K, ld = 2K.  act: NNCV_B200_ACT_*; SiLU and sigmoid of gates below zero are right down to fp32's
+ * smallest numbers, of 16-bit gates to (|gate| + 6) * 2^-22 of the value.  out and scale as above; out may be gate or up where ld is K and the
  * types agree. */
 int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, void* out, int out_dtype, float* scale, int dtype, int M, int K,
                                int act, void* stream);

@@ -9,6 +9,8 @@
 // columns apart, so that what the eight load and store at once lies in a row.  (Eight values a thread, a 64-bit division for each block
 // and a test for infinities for each value took twice the time.)  Of the 6.5 TB/s of a copy: norm 4096 x 4096 bf16 with residual to e4m3 5.9
 // (19.8 us), gated SiLU 2048 x 8192 bf16 to e4m3 6.1 (13.7 us), 8192 x 2048 bf16 to e4m3 5.6 (9.0 us), 4096 x 4096 fp32 in blocks 5.9 (14.3 us).
+#include <type_traits>
+
 #include "activation.cuh"
 #include "epilogue.cuh"
 #include "kernels.h"
@@ -167,11 +169,39 @@ __device__ __forceinline__ void put_block(uint8_t* row, float* scale, int col0, 
 }
 
 // x / (1 + exp(-x)) on the hardware's exponential and reciprocal: exp is off by 2 steps of fp32 and by what rounding x * log2(e) makes of
-// it, far below half a step of the 16-bit values that come in.  exp(-x) = inf gives 0, or NaN for -inf, as the quotient does.
+// it, far below half a step of the 16-bit values that come in.
 __device__ __forceinline__ float silu16(float x) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
   return x * reciprocal(1.0f + e);
+}
+// SiLU and sigmoid have far gates: beyond kFar, 1 + exp(-|x|) is 1, and below -kFar x / (1 + exp(-x)) is x exp(x).  exp(-x) passes fp32's range from
+// -88.7 on, and the hardware's reciprocal is 0 from -87.3 on, where the result is no zero yet and a large `up` makes an ordinary value of it.
+constexpr float kFar = 80.0f;
+template <typename T> __device__ __forceinline__ bool any_far(const Raw<T>& r) {   // NaN is passed over
+  const T* e = reinterpret_cast<const T*>(r.p);
+  if constexpr (sizeof(T) == 4) {
+    float a = fabsf(e[0]);
+#pragma unroll
+    for (int i = 1; i < kV; ++i) a = fmaxf(a, fabsf(e[i]));
+    return a > kFar;
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* p = reinterpret_cast<const T2*>(e);
+    T2 a = __habs2(p[0]);
+#pragma unroll
+    for (int i = 1; i < kV / 2; ++i) a = __hmax2(a, __habs2(p[i]));
+    return fmaxf(ef<T>(a.x), ef<T>(a.y)) > kFar;
+  }
+}
+template <bool SILU>
+__device__ __forceinline__ float far_gate(float x) {
+  const float h = expf(0.5f * x);
+  return x > 0.0f ? (SILU ? x : 1.0f) : (SILU ? x * h : h) * h;
+}
+template <typename T, int ACT>
+__device__ __forceinline__ float near_gate(float x, int act) {
+  return ACT == kActSilu && sizeof(T) == 2 ? silu16(x) : activate<sizeof(T) == 2>(x, ACT < 0 ? act : ACT);
 }
 
 // ---------------------------------------------------------------- root-mean-square norm ----
@@ -288,12 +318,39 @@ rmsnorm_long_kernel(const T* x, long long ldx, const T* residual, const float* w
 }
 
 // ---------------------------------------------------------------- (gated) activation -------
+// What a warp does whose blocks have a far gate, value by value through local memory: unrolled it took 20 registers of the kernel below, which lost a
+// third of its warps.
+template <typename T, bool Q, int ACT>
+__device__ __forceinline__ void gated_far(const T* gate, const T* up, void* out, float* scale, int col0, int t, int K, int act) {
+  float z[kV];
+#pragma unroll 1
+  for (int e = 0; e < kV; ++e) {
+    const int col = col0 + piece_col(e / kPiece, t) + e % kPiece;
+    const float x = col < K ? ef<T>(gate[col]) : 0.0f;
+    float y = fabsf(x) > kFar ? (act == kActSilu ? far_gate<true>(x) : far_gate<false>(x)) : near_gate<T, ACT>(x, act);
+    if (up) y *= col < K ? ef<T>(up[col]) : 0.0f;
+    z[e] = col < K ? y : 0.0f;
+  }
+  float v[kV];
+#pragma unroll
+  for (int e = 0; e < kV; ++e) v[e] = z[e];
+  if (Q) put_block<false>(static_cast<uint8_t*>(out), scale, col0, t, K, v);
+  else store_row<T, false>(static_cast<T*>(out), col0, t, K, v);
+}
+// The same as a call.  The kernel is faster around one but from 16 bits to e4m3 (2048 x 8192, call and body in place: sigmoid fp32 30.5 and 37.5 us,
+// bf16 15.9 and 20.7, to e4m3 23.4 and 20.6).
+template <typename T, bool Q, int ACT>
+__device__ __noinline__ void gated_far_call(const T* gate, const T* up, void* out, float* scale, int col0, int t, int K, int act) {
+  gated_far<T, Q, ACT>(gate, up, out, scale, col0, t, K, act);
+}
+
 // A thread has its part of one block, of two where there is a single tensor: then as many bytes are under way (two of two tensors: 16.5 us
-// for 13.7; one of one: 9.7 for 9.0).  ACT: the activation, or -1 for the one in `act`.
+// for 13.7; one of one: 9.7 for 9.0).  With two tensors of 16 bits six CTAs have room at once (40 registers a thread; left to itself with 60,
+// SiLU 2048 x 8192 bf16 to e4m3 takes 16.7 us for 14.4).  ACT: the activation, or -1 for the one in `act`.
 constexpr int kGatedThreads = 256, kGatedBlocks = kGatedThreads / kLanes;
 template <typename T, bool VEC, bool Q, bool UP, int ACT>
-__global__ void __launch_bounds__(kGatedThreads) gated_kernel(const T* gate, const T* up, long long ld, void* out, float* scale, uint32_t blocks,
-                                                              epi::FastDiv kb, int K, int act) {
+__global__ void __launch_bounds__(kGatedThreads, VEC && UP && sizeof(T) == 2 ? 6 : 0)
+gated_kernel(const T* gate, const T* up, long long ld, void* out, float* scale, uint32_t blocks, epi::FastDiv kb, int K, int act) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   constexpr int kUnroll = UP ? 1 : 2;
@@ -312,10 +369,18 @@ __global__ void __launch_bounds__(kGatedThreads) gated_kernel(const T* gate, con
   }
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
+    if ((ACT == kActSilu || (ACT < 0 && (act == kActSilu || act == kActSigmoid))) && __any_sync(0xffffffffu, any_far<T>(g[i]))) {
+      const T *far_gate = gate + row[i] * ld, *far_up = UP ? up + row[i] * ld : nullptr;
+      void* to = static_cast<uint8_t*>(out) + row[i] * K * (Q ? 1 : (long long)sizeof(T));
+      float* to_scale = Q ? scale + row[i] * kb.d + col0[i] / kGroup : nullptr;
+      if (!VEC || !Q || sizeof(T) == 4) gated_far_call<T, Q, ACT>(far_gate, far_up, to, to_scale, col0[i], t, K, act);
+      else gated_far<T, Q, ACT>(far_gate, far_up, to, to_scale, col0[i], t, K, act);
+      continue;
+    }
     float v[kV];
     to_float<T>(g[i], v);
 #pragma unroll
-    for (int e = 0; e < kV; ++e) v[e] = ACT == kActSilu && sizeof(T) == 2 ? silu16(v[e]) : activate<sizeof(T) == 2>(v[e], ACT < 0 ? act : ACT);
+    for (int e = 0; e < kV; ++e) v[e] = near_gate<T, ACT>(v[e], act);
     if (UP) {
       float w[kV];
       to_float<T>(u[i], w);

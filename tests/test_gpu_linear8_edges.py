@@ -88,6 +88,67 @@ def test_gated_to_e4m3_is_the_quotient(with_up):
     assert torch.equal(s.cpu(), want_s) and R.exactly(out, want)
 
 
+# ---------------------------------------------------------------------------------------------------------------- gates far below zero
+def far_gates(dt):
+    x = torch.linspace(-120.0, -70.0, 2048, dtype=torch.float64)
+    return torch.cat([x, -x[:512], torch.linspace(-3.0, 3.0, 512, dtype=torch.float64)]).to(DT[dt]).cuda().view(3, 1024)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("size", [1.0, 1e30, 1e38])
+@pytest.mark.parametrize("pad", [0, 5])
+def test_gates_far_below_zero(dt, act, size, pad):
+    """act(gate) is a small number there and no zero, and a large `up` makes an ordinary value of it.  In fp32 with an exponential of 2 ulp: ten
+    steps in all where the activation is a normal number, half a step of the subnormals (times up) below."""
+    gate = torch.zeros((3, 1024 + pad), device="cuda", dtype=DT[dt])
+    gate[:, :1024] = far_gates(dt)
+    up = torch.full_like(gate, size)
+    gate, up = gate[:, :1024], up[:, :1024]
+    a = R.act(gate, act)
+    y = a * up.double()
+    y = torch.where(y.abs() > torch.finfo(DT[dt]).max, torch.copysign(torch.full_like(y, INF), y), y)
+    out, _ = run_gated(gate, up, act, dt, False)
+    off = 12 * U * y.abs() + 2 * 2.0 ** -149 * up.double().abs()
+    fin = y.isfinite()
+    assert torch.equal(out.double()[~fin], y[~fin])
+    assert ((out.double() - y).abs()[fin] <= (off + R.HALF[DT[dt]] * 1.001 * (y.abs() + off) + R.TINY[DT[dt]])[fin]).all()
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("k", [512, 515])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("with_up", [True, False])
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_a_far_gate_leaves_the_rest_as_it_is(dt, k, act, with_up, e4m3):
+    g = gen(72, dt, k)
+    gate, up = (torch.randn((40, k), generator=g, device="cuda").to(DT[dt]) for _ in range(2))
+    gate[:, ::128] = 3.0
+    up[:, ::128] = 50.0                          # with up the largest value of every block
+    want = run_gated(gate, up if with_up else None, act, dt, e4m3)
+    far = torch.rand((40, k), generator=g, device="cuda") < 0.01
+    far[:, ::128] = False
+    other = gate.clone()
+    other[far] = -95.0
+    # without up a gate beyond 3 may be a block's largest value; where that becomes a far one, the block has another scale
+    y = R.act(gate, act) * (up.double() if with_up else 1)
+    same = R.scales_of(y, 1) == R.scales_of(torch.where(far, 0.0, y), 1)
+    assert same.float().mean() > 0.95 and (same.all() or not with_up)
+    rest = ~far & (same.repeat_interleave(128, 1)[:, :k] if e4m3 else True)
+    for place in ("apart", "gate", "up"):
+        if place == "apart" or e4m3 or (place == "up" and not with_up):
+            got = run_gated(other, up if with_up else None, act, dt, e4m3)
+        else:
+            a, b = other.clone(), up.clone()
+            o = {"gate": a, "up": b}[place]
+            check(lib().nncv_b200_gated_activation(p(a), p(b) if with_up else None, 0, p(o), dt, None, dt, 40, k, ACT[act], stream()))
+            status()
+            got = (o, None)
+        assert torch.equal(got[0].float()[rest], want[0].float()[rest])
+        assert (got[0].float()[far].abs() <= 1e-30).all()
+        assert not e4m3 or torch.equal(got[1][same], want[1][same])
+
+
 # ---------------------------------------------------------------------------------------------------------------- several sizes in one graph
 def test_products_of_several_heights_in_one_graph():
     """Fewer rows take less shared memory: neither a later node of the graph nor a call between its capture and its replay takes
