@@ -357,9 +357,9 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
  * the last block of a row may be shorter.
  * Rows of x, gate and up may lie further apart than K (ldx, ld: elements from row to row, 0 = K); all else is dense.  M = 0 is
  * a call that does nothing; no row, and no side of a product, is longer than 2^30.  All pointers belong to the current device.
- * Everything computes in fp32; an fp16 result beyond its range becomes +-65504.  The norm, the activation and the quantisation take
- * any K up to that and any address of an element; with K a multiple of 8 and everything on 16-byte boundaries they read 16 bytes
- * at a time.
+ * Everything computes in fp32; a finite result beyond fp16's range becomes +-65504 there, an infinite one stays.  The norm, the activation
+ * and the quantisation take any K up to that and any address of an element; with K a multiple of 8 and everything on 16-byte boundaries
+ * they read 16 bytes at a time.
  * The library's first call on a device sets it up and cannot be captured into a graph (nncv_b200_device_status() is one that will do);
  * after it any call of these four can.
  *

@@ -58,6 +58,18 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16, bool rel
   return relu ? ptx::pack_half2_sat_relu(a, b) : ptx::pack_half2_sat(a, b);
 }
 
+// The same to fp16 with infinite values that stay infinite: one beyond 65504 is infinity.
+__device__ __forceinline__ uint32_t pack_half2_inf(float a, float b) {
+  return ptx::pack_half2_sat(a, b) + (fabsf(a) == INFINITY ? 1u : 0u) + (fabsf(b) == INFINITY ? 0x10000u : 0u);
+}
+// Gathers in t, zero at first, whether a value is infinite or NaN: one instruction for two.
+__device__ __forceinline__ void seek_inf(float a, float b, unsigned long long& t) { t = fma2(pk(a, b), 0ull, t); }
+__device__ __forceinline__ bool found_inf(unsigned long long t) {
+  float a, b;
+  unpk(t, a, b);
+  return !(a + b == 0.0f);
+}
+
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));

@@ -86,24 +86,32 @@ __device__ __forceinline__ void store_slab(const GeParams& p, const CUtensorMap*
     const uint32_t buf = stage + turn * epi::kBufBytes, at = buf + (uint32_t)lane * 128u;
     if (lane == 0) ptx::bulk_wait_read<kBufs - 1>();   // the copy that last read this buffer is done
     __syncwarp();
+    unsigned long long seek = 0;
+    auto put = [&](bool inf) {
 #pragma unroll
-    for (int h = 0; h < kSlab / 8; ++h) {   // eight columns
-      float v[8];
+      for (int h = 0; h < kSlab / 8; ++h) {   // eight columns
+        float v[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) epi::unpk(sum[c / 2 + h * 4 + i], v[2 * i], v[2 * i + 1]);
-      if (!PLAIN) bias_relu(p, col + c + h * 8, v);
-      if (kF) {
+        for (int i = 0; i < 4; ++i) epi::unpk(sum[c / 2 + h * 4 + i], v[2 * i], v[2 * i + 1]);
+        if (!PLAIN) bias_relu(p, col + c + h * 8, v);
+        if (kF) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-          epi::sts128(at + ((uint32_t)(2 * h + q) ^ sw) * 16u, __float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
-                      __float_as_uint(v[4 * q + 3]));
-      } else {
-        uint32_t o[4];
+          for (int q = 0; q < 2; ++q)
+            epi::sts128(at + ((uint32_t)(2 * h + q) ^ sw) * 16u, __float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
+                        __float_as_uint(v[4 * q + 3]));
+        } else {
+          uint32_t o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = epi::pack16(v[2 * i], v[2 * i + 1], TYPE == kBF16, false);
-        epi::sts128(at + ((uint32_t)h ^ sw) * 16u, o[0], o[1], o[2], o[3]);
+          for (int i = 0; i < 4; ++i) {
+            if (TYPE == kF16 && !inf) epi::seek_inf(v[2 * i], v[2 * i + 1], seek);
+            o[i] = inf ? epi::pack_half2_inf(v[2 * i], v[2 * i + 1]) : epi::pack16(v[2 * i], v[2 * i + 1], TYPE == kBF16, false);
+          }
+          epi::sts128(at + ((uint32_t)h ^ sw) * 16u, o[0], o[1], o[2], o[3]);
+        }
       }
-    }
+    };
+    put(false);
+    if (TYPE == kF16 && epi::found_inf(seek)) put(true);   // infinite values stay infinite (asked for every eight columns: 4 % of a product, now 1)
     if (p.vec) {
       ptx::fence_proxy_async_smem();
       __syncwarp();
@@ -519,13 +527,16 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           for (int j = 0; j < 4 && n + j < p.N; ++j) to[j] = v[j];
       } else {
         uint16_t* to = static_cast<uint16_t*>(p.C) + o;
-        const uint32_t lo = epi::pack16(v[0], v[1], p.c_type == kBF16, false), hi = epi::pack16(v[2], v[3], p.c_type == kBF16, false);
-        if (p.vec) *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+        uint32_t h[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          h[j] = p.c_type == kBF16 ? epi::pack16(v[2 * j], v[2 * j + 1], true, false) : epi::pack_half2_inf(v[2 * j], v[2 * j + 1]);
+        if (p.vec) *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
         else {
-          to[0] = (uint16_t)lo;
-          if (n + 1 < p.N) to[1] = (uint16_t)(lo >> 16);
-          if (n + 2 < p.N) to[2] = (uint16_t)hi;
-          if (n + 3 < p.N) to[3] = (uint16_t)(hi >> 16);
+          to[0] = (uint16_t)h[0];
+          if (n + 1 < p.N) to[1] = (uint16_t)(h[0] >> 16);
+          if (n + 2 < p.N) to[2] = (uint16_t)h[1];
+          if (n + 3 < p.N) to[3] = (uint16_t)(h[1] >> 16);
         }
       }
     }

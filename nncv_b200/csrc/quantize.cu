@@ -55,14 +55,35 @@ __device__ __forceinline__ void to_float(const Raw<T>& r, float (&v)[kV]) {
 #pragma unroll
   for (int i = 0; i < kV; ++i) v[i] = ef<T>(e[i]);
 }
+// A piece in its type.
+template <typename T>
+__device__ __forceinline__ void to_type(const float* v, T* e) {
+#pragma unroll
+  for (int i = 0; i < kPiece; ++i) e[i] = et<T>(v[i]);
+}
+// fp16: finite values beyond its range become +-65504, infinite ones stay.  The plain conversion makes both infinite, so a piece that has none of
+// them needs no second look (looked at one by one, wide norms took a quarter longer).
+template <>
+__device__ __forceinline__ void to_type<__half>(const float* v, __half* e) {
+  __half2* o = reinterpret_cast<__half2*>(e);
+  __half2 most = __half2half2(__ushort_as_half(0));
+#pragma unroll
+  for (int i = 0; i < kPiece / 2; ++i) {
+    o[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    most = __hmax2(most, __habs2(o[i]));   // a NaN is passed over
+  }
+  if (fmaxf(__low2float(most), __high2float(most)) == INFINITY) {
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) e[i] = __ushort_as_half((unsigned short)epi::pack_half2_inf(v[i], 0.0f));
+  }
+}
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_row(T* row, int col0, int t, int K, const float (&v)[kV]) {
 #pragma unroll
   for (int i = 0; i < kV / kPiece; ++i) {
     const int col = col0 + piece_col(i, t);
     alignas(16) T e[kPiece];
-#pragma unroll
-    for (int j = 0; j < kPiece; ++j) e[j] = et<T>(v[i * kPiece + j]);
+    to_type<T>(v + i * kPiece, e);
     if (VEC) {
       if (col < K) {
 #pragma unroll
@@ -279,7 +300,7 @@ rmsnorm_kernel(const T* x, long long ldx, const T* residual, const float* weight
 // or the residual.
 constexpr int kLongThreads = 512;
 template <typename T, bool VEC, bool Q>
-__global__ void __launch_bounds__(kLongThreads)
+__global__ void __launch_bounds__(kLongThreads, VEC && sizeof(T) == 2 ? 2 : 0)
 rmsnorm_long_kernel(const T* x, long long ldx, const T* residual, const float* weight, float eps, T* sum, void* out, float* scale, int K) {
   __shared__ float s_part[32];
   const int t = threadIdx.x & (kLanes - 1), first = (int)threadIdx.x / kLanes * kGroup, step = kLongThreads / kLanes * kGroup, kb = (K + kGroup - 1) / kGroup;

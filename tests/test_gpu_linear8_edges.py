@@ -149,6 +149,77 @@ def test_a_far_gate_leaves_the_rest_as_it_is(dt, k, act, with_up, e4m3):
         assert not e4m3 or torch.equal(got[1][same], want[1][same])
 
 
+# ---------------------------------------------------------------------------------------------------------------- infinities in 16 bits
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("k", [512, 515, 16400, 16403])
+def test_norm_keeps_infinities(dt, k):
+    """The sum with the residual is itself infinite, not the type's largest value; the row's norm is 1 / inf."""
+    g = gen(81, dt, k)
+    x, r = (torch.randn((6, k), generator=g, device="cuda").to(DT[dt]) for _ in range(2))
+    x[0, 3], x[1, k - 1], r[2, 200], x[3, 7], x[4, 9], r[4, 9] = INF, -INF, INF, NAN, INF, -INF
+    want = x.double() + r.double()
+    for e4m3 in (False, True):
+        out, sums, s = run_norm(x, r, None, 1e-6, dt, e4m3, True)
+        assert torch.equal(sums.double().isnan(), want.isnan())
+        bad = want.isinf()
+        assert bad.sum() == 3 and torch.equal(sums.double()[bad], want[bad])
+        v = out.float()
+        assert torch.isnan(v[3]).all() and torch.isnan(v[4]).all() and torch.isfinite(v[5]).all()
+        for row in range(3):
+            assert torch.isnan(v[row][bad[row]]).all() and (v[row][~bad[row]] == 0).all()
+    big = torch.full((1, k), 60000.0 if dt == F16 else 1.0, device="cuda").to(DT[dt])
+    _, sums, _ = run_norm(big, big, None, 1e-6, dt, False, True)
+    assert (sums == (65504 if dt == F16 else 2)).all()      # what is finite stays finite
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("k", [512, 515])
+@pytest.mark.parametrize("act", ["none", "silu", "hard_swish"])
+@pytest.mark.parametrize("with_up", [True, False])
+def test_gated_keeps_infinities(dt, k, act, with_up):
+    g = gen(82, dt, k)
+    gate, up = (torch.randn((6, k), generator=g, device="cuda").to(DT[dt]) for _ in range(2))
+    up = up.abs() + 0.25
+    gate[0, 3], gate[1, k - 1], gate[2, 130] = INF, NAN, 200.0
+    up[2, 130], up[3, 5], up[4, 6] = (65504.0 if dt == F16 else 2.0), NAN, INF
+    gate[4, 6] = 2.0
+    out, _ = run_gated(gate, up if with_up else None, act, dt, False)
+    assert out[0, 3] == INF and torch.isnan(out[1, k - 1])
+    assert out[2, 130] == ((65504 if dt == F16 else 400) if with_up else 200)
+    bad = [(0, 3), (1, k - 1)]
+    if with_up:
+        assert torch.isnan(out[3, 5]) and out[4, 6] == INF
+        bad += [(3, 5), (4, 6)]
+    q, s = run_gated(gate, up if with_up else None, act, dt, True)
+    v = R.dequantize(q, s, 1)
+    for t in (out, v):
+        fin = torch.ones_like(t, dtype=torch.bool)
+        for at in bad:
+            fin[at] = False
+        assert torch.isfinite(t[fin]).all()
+    assert all(torch.isnan(v[at]) for at in bad) and torch.isfinite(s).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 64, 2048), (40, 264, 256), (40, 261, 256), (776, 5000, 640), (2304, 2304, 1152), (1600, 1999, 2000)])
+@pytest.mark.parametrize("cdt", [F32, F16, BF16])
+@pytest.mark.parametrize("epilogue", [False, True])
+def test_matmul_keeps_infinities(m, n, k, cdt, epilogue):
+    """An infinite scale makes its row infinite in every type; what is finite but beyond fp16 becomes its largest value."""
+    g = gen(83, m, n, k)
+    a, sa = R.operand(g, m, k, 1)
+    b, sb = R.operand(g, n, k, 128)
+    a.view(torch.uint8).bitwise_and_(0x7F)   # no negative values, so that no row adds infinities of both signs
+    b.view(torch.uint8).bitwise_and_(0x7F)
+    sa[1, 0] = INF
+    sa[2] *= 1e7
+    bias = torch.randn(n, generator=g, device="cuda") if epilogue else None
+    c = run_matmul(a, sa, b, sb, cdt, bias, epilogue)
+    assert (c[1] == INF).all()
+    assert (c[2] == 65504).all() if cdt == F16 else torch.isfinite(c[2]).all()
+    rest = [i for i in range(m) if i not in (1, 2)]
+    assert torch.isfinite(c[rest]).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------- several sizes in one graph
 def test_products_of_several_heights_in_one_graph():
     """Fewer rows take less shared memory: neither a later node of the graph nor a call between its capture and its replay takes
