@@ -367,7 +367,8 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
  *   x [M,K] of dtype; residual [M,K] of dtype or NULL; weight fp32 [K] or NULL (= 1)
  *   sum: NULL, or [M,K] of dtype that receives h (the norm is taken of h before this rounding); may be residual, or x where ldx is K
  *   out: [M,K] of out_dtype, which is dtype or NNCV_B200_E4M3; scale: fp32 [M, ceil(K/128)] with E4M3, else NULL
- * out may be x (where ldx is K) or residual, if it has their type.  A row whose squares' sum passes fp32's range gives zeros. */
+ * out may be x (where ldx is K) or residual, if it has their type.  A row whose squares' sum passes fp32's range gives
+ * zeros; of one whose squares are too small for it (values below 1e-22) the root of eps is all there is to divide by. */
 int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const void* weight, float eps, void* sum, void* out, int out_dtype,
                       float* scale, int dtype, int M, int K, void* stream);
 /* out = activation(gate) * up, or activation(gate) where up is NULL.  gate and up [M,K] of dtype, rows ld apart: the halves of one

@@ -290,7 +290,7 @@ rmsnorm_kernel(const T* x, long long ldx, const T* residual, const float* weight
     const float norm = 1.0f / sqrtf(cta_sum(ss, s_part[turn]) / (float)K + eps);
     if (!kKeep) load_weight<VEC>(weight, col0, t, K, w);
 #pragma unroll
-    for (int e = 0; e < kV; ++e) h[e] *= norm * w[e];
+    for (int e = 0; e < kV; ++e) h[e] = h[e] * norm * w[e];   // the row is of size one before the weight comes
     if (Q) put_block<VEC>(static_cast<uint8_t*>(out) + row * K, scale + row * kb + col0 / kGroup, col0, t, K, h);
     else store_row<T, VEC>(static_cast<T*>(out) + row * K, col0, t, K, h);
   }
@@ -332,7 +332,7 @@ rmsnorm_long_kernel(const T* x, long long ldx, const T* residual, const float* w
     if (residual) add_raw<T>(b, h);
     if (sum) store_row<T, VEC>(sum + row * K, col0, t, K, h);
 #pragma unroll
-    for (int e = 0; e < kV; ++e) h[e] *= norm * w[e];
+    for (int e = 0; e < kV; ++e) h[e] = h[e] * norm * w[e];   // the row is of size one before the weight comes
     if (Q) put_block<VEC>(static_cast<uint8_t*>(out) + row * K, scale + row * kb + col0 / kGroup, col0, t, K, h);
     else store_row<T, VEC>(static_cast<T*>(out) + row * K, col0, t, K, h);
   }

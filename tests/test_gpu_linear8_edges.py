@@ -220,6 +220,19 @@ def test_matmul_keeps_infinities(m, n, k, cdt, epilogue):
     assert torch.isfinite(c[rest]).all()
 
 
+# ---------------------------------------------------------------------------------------------------------------- weights far from one
+@pytest.mark.parametrize("k", [512, 9000, 16400])
+@pytest.mark.parametrize("size,weight", [(1e16, 1e-25), (1e-16, 1e24), (1e15, 1e-30)])
+def test_norm_with_weights_far_from_one(k, size, weight):
+    """The row is brought to size one before the weight comes: neither passes fp32's range."""
+    x = torch.randn((3, k), generator=gen(91, k), device="cuda") * size
+    w = (torch.randn(k, generator=gen(92, k), device="cuda") + 2) * weight
+    out, _, _ = run_norm(x, None, w, 0.0, F32, False, False)
+    h = x.double()
+    y = h / torch.sqrt((h * h).mean(1, keepdim=True)) * w.double()
+    assert ((out.double() - y).abs() <= 50 * U * y.abs()).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------- several sizes in one graph
 def test_products_of_several_heights_in_one_graph():
     """Fewer rows take less shared memory: neither a later node of the graph nor a call between its capture and its replay takes
