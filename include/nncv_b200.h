@@ -356,7 +356,8 @@ int nncv_b200_upsample2x_nhwc(const void* in, void* out, int dtype, int N, int H
  * [M, ceil(K/128)] (activations: one for 128 columns of a row) or [ceil(M/128), ceil(K/128)] (weights: one for 128 x 128), row-major;
  * the last block of a row may be shorter.
  * Rows of x, gate and up may lie further apart than K (ldx, ld: elements from row to row, 0 = K); all else is dense.  M = 0 is
- * a call that does nothing; no row, and no side of a product, is longer than 2^30.  All pointers belong to the current device.
+ * a call that does nothing, whatever the addresses of the tensors with M rows; no row, and no side of a product, is longer than
+ * 2^30.  All pointers belong to the current device.
  * Everything computes in fp32; a finite result beyond fp16's range becomes +-65504 there, an infinite one stays.  The norm, the activation
  * and the quantisation take any K up to that and any address of an element; with K a multiple of 8 and everything on 16-byte boundaries
  * they read 16 bytes at a time.

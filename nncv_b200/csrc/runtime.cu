@@ -3090,9 +3090,17 @@ static bool of_type(const void* p, int dtype) { return on_boundary(p, dtype_size
 // columns, and blocks of 128 of them, are counted in 31 bits with room for a last step beyond the end
 constexpr int kMostColumns = 1 << 30;
 static bool too_large(int M, int K) { return K > kMostColumns || (long long)M * (((long long)K + 127) / 128) > 0x7fffff00LL; }
-// out_dtype is dtype or E4M3, and scales go with E4M3 alone
-static int check_out(const char* what, int out_dtype, int dtype, const void* out, const float* scale) {
+static int check_out_type(const char* what, int out_dtype, int dtype) {
   if (out_dtype != dtype && out_dtype != NNCV_B200_E4M3) return fail(NNCV_B200_EINVAL, "%s: out_dtype must be dtype or E4M3", what);
+  return NNCV_B200_OK;
+}
+// A call on tensors without rows does nothing, and asks for no addresses: such tensors have no memory.
+static int no_rows() {
+  const int rc = device_init();
+  return rc ? rc : ok();
+}
+// scales go with E4M3 alone
+static int check_out(const char* what, int out_dtype, int dtype, const void* out, const float* scale) {
   if ((out_dtype == NNCV_B200_E4M3) != (scale != nullptr)) return fail(NNCV_B200_EINVAL, "%s: scale goes with an E4M3 result, and only with one", what);
   if ((out_dtype != NNCV_B200_E4M3 && !of_type(out, dtype)) || !on_boundary(scale, 4)) return fail(NNCV_B200_EINVAL, "%s: a pointer is not on its type's boundary", what);
   return NNCV_B200_OK;
@@ -3102,16 +3110,19 @@ int nncv_b200_rmsnorm(const void* x, long long ldx, const void* residual, const 
                       float* scale, int dtype, int M, int K, void* stream) {
   std::lock_guard<std::mutex> lk(g_mutex);
   int rc = NNCV_B200_OK;
-  if (!x || !out || M < 0 || K <= 0 || dtype < 0 || dtype > 2 || !(eps >= 0.0f)) return fail(NNCV_B200_EINVAL, "rmsnorm: bad argument");
+  if (M < 0 || K <= 0 || dtype < 0 || dtype > 2 || !(eps >= 0.0f)) return fail(NNCV_B200_EINVAL, "rmsnorm: bad argument");
   if (ldx == 0) ldx = K;
   if (ldx < K) return fail(NNCV_B200_EINVAL, "rmsnorm: ldx is less than K");
   if (too_large(M, K)) return fail(NNCV_B200_EINVAL, "rmsnorm: more than 2^30 columns or 2^31 blocks of 128");
+  if ((rc = check_out_type("rmsnorm", out_dtype, dtype))) return rc;
+  if (M == 0) return no_rows();
+  if (!x || !out) return fail(NNCV_B200_EINVAL, "rmsnorm: x and out must not be null");
   if (!of_type(x, dtype) || !of_type(residual, dtype) || !of_type(sum, dtype) || !on_boundary(weight, 4))
     return fail(NNCV_B200_EINVAL, "rmsnorm: a pointer is not on its type's boundary");
   if ((rc = check_out("rmsnorm", out_dtype, dtype, out, scale))) return rc;
   if (ldx != K && (sum == x || out == x)) return fail(NNCV_B200_EINVAL, "rmsnorm: a result may take the place of x only where ldx is K");
   if (out == sum || (out_dtype == NNCV_B200_E4M3 && (out == x || out == residual))) return fail(NNCV_B200_EINVAL, "rmsnorm: out needs memory of its own");
-  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  if ((rc = device_init())) return rc;
   RmsNormArgs a;
   a.x = x; a.ldx = ldx; a.residual = residual; a.weight = (const float*)weight; a.eps = eps; a.sum = sum; a.out = out; a.scale = scale;
   a.dtype = (DType)dtype; a.to_e4m3 = out_dtype == NNCV_B200_E4M3; a.M = M; a.K = K; a.sm_count = g_dev.sm_count;
@@ -3123,15 +3134,18 @@ int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, v
                                int act, void* stream) {
   std::lock_guard<std::mutex> lk(g_mutex);
   int rc = NNCV_B200_OK;
-  if (!gate || !out || M < 0 || K <= 0 || dtype < 0 || dtype > 2 || act < 0 || act > 5) return fail(NNCV_B200_EINVAL, "gated_activation: bad argument");
+  if (M < 0 || K <= 0 || dtype < 0 || dtype > 2 || act < 0 || act > 5) return fail(NNCV_B200_EINVAL, "gated_activation: bad argument");
   if (ld == 0) ld = K;
   if (ld < K) return fail(NNCV_B200_EINVAL, "gated_activation: ld is less than K");
   if (too_large(M, K)) return fail(NNCV_B200_EINVAL, "gated_activation: more than 2^30 columns or 2^31 blocks of 128");
+  if ((rc = check_out_type("gated_activation", out_dtype, dtype))) return rc;
+  if (M == 0) return no_rows();
+  if (!gate || !out) return fail(NNCV_B200_EINVAL, "gated_activation: gate and out must not be null");
   if (!of_type(gate, dtype) || !of_type(up, dtype)) return fail(NNCV_B200_EINVAL, "gated_activation: a pointer is not on its type's boundary");
   if ((rc = check_out("gated_activation", out_dtype, dtype, out, scale))) return rc;
   if ((out == gate || out == up) && (ld != K || out_dtype == NNCV_B200_E4M3))
     return fail(NNCV_B200_EINVAL, "gated_activation: the result may take the place of gate or up only where ld is K and the types agree");
-  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  if ((rc = device_init())) return rc;
   GatedArgs a;
   a.gate = gate; a.up = up; a.ld = ld; a.out = out; a.scale = scale; a.dtype = (DType)dtype; a.to_e4m3 = out_dtype == NNCV_B200_E4M3;
   a.M = M; a.K = K; a.act = act; a.sm_count = g_dev.sm_count;
@@ -3142,14 +3156,16 @@ int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, v
 int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, float* scale, int M, int K, int block_rows, void* stream) {
   std::lock_guard<std::mutex> lk(g_mutex);
   int rc = NNCV_B200_OK;
-  if (!x || !q || !scale || M < 0 || K <= 0 || dtype < 0 || dtype > 2) return fail(NNCV_B200_EINVAL, "quantize_e4m3: bad argument");
+  if (M < 0 || K <= 0 || dtype < 0 || dtype > 2) return fail(NNCV_B200_EINVAL, "quantize_e4m3: bad argument");
   if (block_rows != 1 && block_rows != 128) return fail(NNCV_B200_EINVAL, "quantize_e4m3: block_rows must be 1 or 128");
   if (ldx == 0) ldx = K;
   if (ldx < K) return fail(NNCV_B200_EINVAL, "quantize_e4m3: ldx is less than K");
   if (too_large(M, K)) return fail(NNCV_B200_EINVAL, "quantize_e4m3: more than 2^30 columns or 2^31 blocks of 128");
+  if (M == 0) return no_rows();
+  if (!x || !q || !scale) return fail(NNCV_B200_EINVAL, "quantize_e4m3: x, q and scale must not be null");
   if (!of_type(x, dtype) || !on_boundary(scale, 4)) return fail(NNCV_B200_EINVAL, "quantize_e4m3: a pointer is not on its type's boundary");
   if (q == x) return fail(NNCV_B200_EINVAL, "quantize_e4m3: q needs memory of its own");
-  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  if ((rc = device_init())) return rc;
   if (block_rows == 128) {
     LAUNCH(launch_quantize_blocks(x, ldx, (DType)dtype, q, scale, M, K, (cudaStream_t)stream));
     return ok();
@@ -3164,15 +3180,17 @@ int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, co
                           const float* bias, int relu, void* stream) {
   std::lock_guard<std::mutex> lk(g_mutex);
   int rc = NNCV_B200_OK;
-  if (!A || !scale_a || !B || !scale_b || !C || M < 0 || N <= 0 || K <= 0) return fail(NNCV_B200_EINVAL, "matmul_e4m3: bad argument");
+  if (!B || !scale_b || M < 0 || N <= 0 || K <= 0) return fail(NNCV_B200_EINVAL, "matmul_e4m3: bad argument");
   if (c_dtype < 0 || c_dtype > 2) return fail(NNCV_B200_EINVAL, "matmul_e4m3: c_dtype must be F32, F16 or BF16");
   if (K % 16 != 0) return fail(NNCV_B200_EINVAL, "matmul_e4m3: K must be a multiple of 16");
   if (M > kMostColumns || N > kMostColumns || K > kMostColumns || ((long long)M + 127) / 128 * (((long long)N + 63) / 64) > 0x3fffffffLL)
     return fail(NNCV_B200_EINVAL, "matmul_e4m3: a side longer than 2^30, or more than 2^30 tiles of 128 x 64");
+  if (M == 0) return no_rows();
+  if (!A || !scale_a || !C) return fail(NNCV_B200_EINVAL, "matmul_e4m3: A, scale_a and C must not be null");
   if (!on_boundary(A, 16) || !on_boundary(B, 16)) return fail(NNCV_B200_EINVAL, "matmul_e4m3: A and B must lie on 16-byte boundaries");
   if (!of_type(C, c_dtype) || !on_boundary(scale_a, 4) || !on_boundary(scale_b, 4) || !on_boundary(bias, 4))
     return fail(NNCV_B200_EINVAL, "matmul_e4m3: a pointer is not on its type's boundary");
-  if ((rc = device_init()) || M == 0) return rc ? rc : ok();
+  if ((rc = device_init())) return rc;
   GemmE4m3Args a;
   a.A = A; a.scale_a = scale_a; a.B = B; a.scale_b = scale_b; a.C = C; a.bias = bias; a.c_dtype = (DType)c_dtype; a.relu = relu;
   a.M = M; a.N = N; a.K = K; a.sm_count = g_dev.sm_count; a.error_flag = g_dev.error_flag;

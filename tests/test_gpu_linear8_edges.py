@@ -233,6 +233,26 @@ def test_norm_with_weights_far_from_one(k, size, weight):
     assert ((out.double() - y).abs() <= 50 * U * y.abs()).all()
 
 
+# ---------------------------------------------------------------------------------------------------------------- empty tensors
+def test_empty_tensors_are_calls_that_do_nothing():
+    """A tensor without rows has no memory: its address is null."""
+    L, n0 = lib(), lib().nncv_b200_launch_count()
+    x = torch.empty((0, 256), device="cuda", dtype=torch.bfloat16)
+    q, s = torch.empty((0, 256), device="cuda", dtype=torch.float8_e4m3fn), torch.empty((0, 2), device="cuda")
+    b, sb = R.operand(gen(6), 64, 256, 128)
+    c = torch.empty((0, 64), device="cuda")
+    assert p(x) == p(q) == p(s) == p(c) == 0
+    check(L.nncv_b200_rmsnorm(p(x), 0, p(x), None, 1e-6, p(x), p(x), BF16, None, BF16, 0, 256, stream()))
+    check(L.nncv_b200_rmsnorm(p(x), 0, p(x), None, 1e-6, p(x), p(q), E4M3, p(s), BF16, 0, 256, stream()))
+    check(L.nncv_b200_gated_activation(p(x), p(x), 0, p(x), BF16, None, BF16, 0, 256, ACT["silu"], stream()))
+    check(L.nncv_b200_gated_activation(p(x), p(x), 0, p(q), E4M3, p(s), BF16, 0, 256, ACT["silu"], stream()))
+    for rows in (1, 128):
+        check(L.nncv_b200_quantize_e4m3(p(x), 0, BF16, p(q), p(s), 0, 256, rows, stream()))
+    check(L.nncv_b200_matmul_e4m3(p(q), p(s), p(b), p(sb), p(c), 0, 64, 256, F32, None, 0, stream()))
+    status()
+    assert L.nncv_b200_launch_count() == n0
+
+
 # ---------------------------------------------------------------------------------------------------------------- several sizes in one graph
 def test_products_of_several_heights_in_one_graph():
     """Fewer rows take less shared memory: neither a later node of the graph nor a call between its capture and its replay takes
