@@ -27,6 +27,7 @@
 
 #include "epilogue.cuh"
 #include "kernels.h"
+#include "pair_copies.h"
 #include "ptx.cuh"
 
 namespace nncv_b200 {
@@ -166,6 +167,8 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   static_assert(kSlots * kSlotBytes <= (uint32_t)kScaleBytes, "");
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_abort;
+  __shared__ int s_gave_up;         // of a pair, in both CTAs: a producer of theirs did
+  __shared__ __align__(8) long long s_issued;   // blocks whose copies this CTA has issued
   __shared__ uint32_t s_tmem;
   __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 3 * kMaxAccs + 1];
   const uint32_t raw = ptx::smem_u32(smem_raw);
@@ -186,6 +189,7 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   const uint32_t rank = PAIR || p.splits_log ? ptx::cluster_ctarank() : 0u;
   if (threadIdx.x == 0) {
     s_abort = 0;
+    s_gave_up = 0;
     for (int i = 0; i < p.stages; ++i) {
       ptx::mbar_init(full + 8 * i, 1);
       ptx::mbar_init(empty + 8 * i, 1);
@@ -253,10 +257,10 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       const uint32_t full_at = PAIR ? ptx::map_to_cta(full, 0) : full;   // the bytes of a stage, of both CTAs, are counted on the leader's barrier
       uint32_t st = 0, ph = 0, used = 0;
       bool okw = true;
-      int m0, n0;
-      for (int i = 0; okw && item(i, m0, n0); ++i) {
+      int m0, n0, i = 0, kb = 0;
+      for (; item(i, m0, n0); ++i) {
         if (PAIR) n0 += (int)rank * (kPartN / 2);   // each CTA brings half of the columns of every part
-        for (int kb = kb_lo; kb < kb_hi; ++kb) {
+        for (kb = kb_lo; kb < kb_hi; ++kb) {
           if (!ptx::warp_wait(empty + 8 * st, ph ^ 1u, abort_flag)) { okw = false; break; }
           const uint32_t dst = ring + st * stage_bytes, dst_b = dst + (uint32_t)p.a_bytes;
           if (PAIR) {
@@ -273,11 +277,20 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           used |= 1u << st;
           if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
         }
+        if (!okw) break;
+        kb = 0;
       }
-      if (!okw) {   // copies in flight land before the CTA ends: the last round of every stage that was used
-        if (!PAIR || rank == 0)
+      if (PAIR && lane == 0) s_issued = (long long)i * p.KB + kb;
+      if (!okw) {   // copies in flight land before the CTA ends: of a pair after both have met, else here the last round of every stage that was used
+        if (PAIR) {
+          if (lane == 0) {
+            s_gave_up = 1;
+            ptx::st_cluster(ptx::map_to_cta(ptx::smem_u32(&s_gave_up), rank ^ 1u), 1u);
+          }
+        } else {
           for (uint32_t j = 0; j < (uint32_t)p.stages; ++j)
             if (used >> j & 1u) ptx::mbar_wait(full + 8 * j, j < st ? ph : ph ^ 1u);
+        }
         if (lane == 0 && p.error_flag) atomicCAS(p.error_flag, 0, (int)kErrWaitProducer);
       }
     } else if (warp == 1) {
@@ -543,7 +556,30 @@ gemm_e4m3_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     __syncwarp();
     ptx::cluster_sync_all();   // the peers' reads of this CTA's partial sums are over
   }
-  if (PAIR) ptx::cluster_sync_all();
+  if (PAIR) {
+    ptx::cluster_sync_all();
+    if (*reinterpret_cast<volatile int*>(&s_gave_up)) {   // in both CTAs; the MMAs have ended
+      if (warp == 0) {
+        const uint32_t issue = ptx::elect_one(), full_at = ptx::map_to_cta(full, 0);
+        const long long mine = *reinterpret_cast<volatile long long*>(&s_issued);
+        const long long end = pair_copies::meet_at(mine, ptx::ld_cluster_s64(ptx::map_to_cta(ptx::smem_u32(&s_issued), rank ^ 1u)));
+        for (long long n = mine; n < end; ++n) {   // nobody reads what these bring
+          const uint32_t st = pair_copies::spot_of(n, p.stages).stage, dst = ring + st * stage_bytes;
+          if (rank == 0) ptx::mbar_arrive_expect_tx(full + 8 * st, 2 * stage_bytes, issue);
+          ptx::tma_load_2d_pair(dst, &tm_a, 0, 0, full_at + 8 * st, issue);
+#pragma unroll
+          for (int h = 0; h < kNS; ++h) ptx::tma_load_2d_pair(dst + (uint32_t)p.a_bytes + h * (kBBytes / kNS), &tm_b, 0, 0, full_at + 8 * st, issue);
+        }
+        if (rank == 0)
+          for (long long n = pair_copies::wait_from(end, p.stages); n < end; ++n) {
+            const pair_copies::Spot at = pair_copies::spot_of(n, p.stages);
+            ptx::mbar_wait(full + 8 * at.stage, at.parity);
+          }
+        __syncwarp();
+      }
+      ptx::cluster_sync_all();
+    }
+  }
   if (warp == 1) {
     __syncwarp();
     if (PAIR) ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
