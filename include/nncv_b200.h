@@ -386,6 +386,11 @@ int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, fl
  * No scratch: calls on several streams, and captured calls, share nothing. */
 int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, const float* scale_b, void* C, int M, int N, int K, int c_dtype,
                           const float* bias, int relu, void* stream);
+/* Force the tile of the products that follow: 0 = 128 x 64, 1 = 128 x 128, each shared by ctas = 1, 2, 4 or 8 CTAs; 2 = 256 x 128 and
+ * 3 = 256 x 256 on CTA pairs, ctas = 1.  What does not fit a product (more tiles than clusters run at once, fewer blocks of K than CTAs)
+ * is chosen as without it; tile -1 restores the built-in choice, less leaves the setting as it is.  Returns tile * 16 + ctas of the last
+ * product, -1 before the first.  A tuning and test hook of the whole library with no counterpart in the reference. */
+int nncv_b200_matmul_e4m3_tile(int tile, int ctas);
 
 #ifdef __cplusplus
 }

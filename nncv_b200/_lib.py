@@ -31,6 +31,7 @@ EXPORTS = [
     "nncv_b200_conv_run_fused", "nncv_b200_conv_set_tile", "nncv_b200_stem_pool", "nncv_b200_stem_variant",
     "nncv_b200_maxpool_nhwc", "nncv_b200_avgpool_nhwc", "nncv_b200_nchw_to_nhwc", "nncv_b200_bn_fold",
     "nncv_b200_rmsnorm", "nncv_b200_gated_activation", "nncv_b200_quantize_e4m3", "nncv_b200_matmul_e4m3",
+    "nncv_b200_matmul_e4m3_tile",
 ]
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
@@ -127,6 +128,7 @@ def lib() -> ctypes.CDLL:
     L.nncv_b200_gated_activation.argtypes = [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
     L.nncv_b200_quantize_e4m3.argtypes = [c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]
     L.nncv_b200_matmul_e4m3.argtypes = [c_void_p] * 5 + [c_int] * 4 + [c_void_p, c_int, c_void_p]
+    L.nncv_b200_matmul_e4m3_tile.argtypes = [c_int, c_int]
     _lib = L
     return L
 

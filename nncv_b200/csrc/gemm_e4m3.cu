@@ -25,6 +25,7 @@
 
 #include <mutex>
 
+#include "e4m3_tile.h"
 #include "epilogue.cuh"
 #include "kernels.h"
 #include "pair_copies.h"
@@ -634,31 +635,13 @@ size_t smem_of(int a_rows, int* stages) {
   return fixed + *stages * stage;
 }
 
-// Tile and CTAs that share a tile's blocks: the least of a model's times, in us: rounds x (blocks x time of one + end of a tile) + launch
-// (+ exchange of partial sums).  A block of 128 takes longer with more rows of A, up to a whole tile.  The constants are fitted to 90
-// shapes (M and N 1 .. 8192, K 16 .. 8192), each timed with every tile and split that fits: the choice is 0.5 % above the fastest on
-// average, 9 % at worst (1024^3: 128 x 64 6.0 us, 256 x 128 on pairs 5.5).
-int pick(int M, int N, int KB, int sms, int* splits) {
-  struct Tile { int m, n; double block, more, round, launch; };
-  static const Tile tiles[4] = {{128, 64, 0.16, 0.11, 0.75, 1.7}, {128, 128, 0.17, 0.20, 1.0, 1.8}, {256, 128, 0.27, 0.0, 1.1, 2.2}, {256, 256, 0.42, 0.0, 2.5, 2.0}};
+// Tile and CTAs that share a tile's blocks: what the caller asks for where that fits, else the model's choice.
+e4m3::Choice pick(const GemmE4m3Args& a, int KB, int sms) {
   int stages;
   static const ClusterFit fit64 = cluster_fit(gemm_e4m3_kernel<64, false>, threads_of(64), smem_of<64, false>(kBM, &stages), sms);
   static const ClusterFit fit128 = cluster_fit(gemm_e4m3_kernel<128, false>, threads_of(128), smem_of<128, false>(kBM, &stages), sms);
-  const double rows = (M < kBM ? M : kBM) / (double)kBM;
-  int best = 0;
-  double least = 1e30;
-  for (int i = 0; i < 4; ++i) {
-    const Tile& t = tiles[i];
-    const long long items = ((long long)M + t.m - 1) / t.m * (((long long)N + t.n - 1) / t.n);
-    for (int s = 1; s <= (i < 2 ? 8 : 1); s *= 2) {
-      const long long slots = i >= 2 ? sms / 2 : s == 1 ? sms : (i == 0 ? fit64 : fit128).of[s];
-      if (s > 1 && (items > slots || KB < s)) break;
-      double us = (double)((items + slots - 1) / slots) * ((KB + s - 1) / s * (t.block + t.more * rows) + t.round) + t.launch;
-      if (s > 1) us += 0.8 + 1.8 * rows * (i + 1);
-      if (us < least) { least = us; best = i; *splits = s; }
-    }
-  }
-  return best;
+  const e4m3::Room room{{fit64.of, fit128.of}, sms};
+  return e4m3::fits(a.tile, a.splits, a.M, a.N, KB, room) ? e4m3::Choice{a.tile, a.splits} : e4m3::choose(a.M, a.N, KB, room);
 }
 
 template <int BN, bool PAIR>
@@ -713,10 +696,11 @@ cudaError_t launch_gemm_e4m3(const GemmE4m3Args& a, cudaStream_t st) {
   p.M = a.M; p.N = a.N; p.KB = (a.K + kBlockK - 1) / kBlockK;
   p.c_type = a.c_dtype; p.relu = a.relu;
   p.vec = (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 && (long long)a.N * (long long)dtype_size(a.c_dtype) % 16 == 0;
-  int splits = 1;
-  switch (pick(a.M, a.N, p.KB, a.sm_count > 0 ? a.sm_count : 148, &splits)) {
-    case 0: return launch_as<64, false>(a, p, splits, st);
-    case 1: return launch_as<128, false>(a, p, splits, st);
+  const e4m3::Choice c = pick(a, p.KB, a.sm_count > 0 ? a.sm_count : 148);
+  if (a.took) *a.took = c.tile * 16 + c.splits;
+  switch (c.tile) {
+    case 0: return launch_as<64, false>(a, p, c.splits, st);
+    case 1: return launch_as<128, false>(a, p, c.splits, st);
     case 2: return launch_as<128, true>(a, p, 1, st);
     default: return launch_as<256, true>(a, p, 1, st);
   }

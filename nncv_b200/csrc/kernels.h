@@ -335,6 +335,8 @@ struct GemmE4m3Args {
   DType c_dtype = kF32;
   int relu = 0;
   int M = 0, N = 0, K = 0;
+  int tile = -1, splits = 0;           // asked for (see e4m3_tile.h), or none
+  int* took = nullptr;                 // tile * 16 + splits of the launch
   int sm_count = 0;
   int* error_flag = nullptr;
 };

@@ -3176,6 +3176,8 @@ int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, fl
   return ok();
 }
 
+static int g_e4m3_tile = -1, g_e4m3_ctas = 0;   // what nncv_b200_matmul_e4m3_tile asks for
+static int g_e4m3_took = -1;
 int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, const float* scale_b, void* C, int M, int N, int K, int c_dtype,
                           const float* bias, int relu, void* stream) {
   std::lock_guard<std::mutex> lk(g_mutex);
@@ -3194,8 +3196,18 @@ int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, co
   GemmE4m3Args a;
   a.A = A; a.scale_a = scale_a; a.B = B; a.scale_b = scale_b; a.C = C; a.bias = bias; a.c_dtype = (DType)c_dtype; a.relu = relu;
   a.M = M; a.N = N; a.K = K; a.sm_count = g_dev.sm_count; a.error_flag = g_dev.error_flag;
+  a.tile = g_e4m3_tile; a.splits = g_e4m3_ctas; a.took = &g_e4m3_took;
   LAUNCH(launch_gemm_e4m3(a, (cudaStream_t)stream));
   return ok();
+}
+
+int nncv_b200_matmul_e4m3_tile(int tile, int ctas) {
+  std::lock_guard<std::mutex> lk(g_mutex);
+  if (tile >= -1) {
+    g_e4m3_tile = tile;
+    g_e4m3_ctas = ctas;
+  }
+  return g_e4m3_took;
 }
 
 }  // extern "C"
