@@ -382,8 +382,10 @@ int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, v
 int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, float* scale, int M, int K, int block_rows, void* stream);
 /* C[M,N] = A * B^T (+ bias[N]) (+ ReLU): A [M,K] e4m3 with scales [M, ceil(K/128)], B [N,K] e4m3 (as a fully connected layer
  * stores its weights) with scales [ceil(N/128), ceil(K/128)]; C of c_dtype F32, F16 or BF16.  K a multiple of 16, A and B on 16-byte
- * boundaries, C on any element's.  fp32 sums; a block's sum is scaled before it is added to the others.  C must not overlap an operand.
- * No scratch: calls on several streams, and captured calls, share nothing. */
+ * boundaries, C on any element's.  fp32 sums; a block's sum is scaled before it is added to the others, by the fp32 product of its
+ * two scales: where that is below 2^-126 the block is off by up to 2^-125, and from 2^128 on it is infinite (NaN where its sum is 0).
+ * The order in which blocks are added goes by M, N, K and the device, so a row's last bits may differ from batch to batch.  C must not
+ * overlap an operand.  No scratch: calls on several streams, and captured calls, share nothing. */
 int nncv_b200_matmul_e4m3(const void* A, const float* scale_a, const void* B, const float* scale_b, void* C, int M, int N, int K, int c_dtype,
                           const float* bias, int relu, void* stream);
 /* Force the tile of the products that follow: 0 = 128 x 64, 1 = 128 x 128, each shared by ctas = 1, 2, 4 or 8 CTAs; 2 = 256 x 128 and

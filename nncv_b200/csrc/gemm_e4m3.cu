@@ -7,8 +7,8 @@
 // out of tensor memory and added, times its scale, to fp32 sums in the registers of the epilogue warps; tensor memory holds the
 // sums of several blocks, and the MMAs of the next ones go on meanwhile.
 // Roles: warp 0 copies, warp 1 issues the MMAs, warps 2 and 3 bring the products of the scales, the others add up and store.
-// Rows and columns behind M and N read as zero and are not stored.  Every wait is bounded and abortable; one that runs out sets
-// the device status word.
+// Columns behind N read as zero, rows behind M as zero or, below 128 rows, as what lies there; neither is stored.  Every wait is bounded
+// and abortable; one that runs out sets the device status word.
 //
 // What bounds it.  Large: the power limit.  A block of a 256 x 256 tile on a CTA pair is 512 clocks of MMAs; copies and MMAs alone take
 // 540, with the sums taken out and scaled 640, with the result's stores 708 on average; the clock falls from 1.97 to 1.3 GHz.

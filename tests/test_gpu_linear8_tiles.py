@@ -101,3 +101,53 @@ def test_rows_of_a_small_batch_and_of_a_large_one(cdt):
         tiles.add(took())
         assert ((part - whole[:m]).abs() <= 2 * bound[:m]).all()
     assert len(tiles) > 2
+
+
+def powers(rows, k, e, spread):
+    """Scales 2^e times a power of two between 1 and 2^spread, by block."""
+    i = torch.arange(rows * R.blocks(k), device="cuda") % (spread + 1)
+    return torch.exp2((e + i).float()).view(rows, R.blocks(k))
+
+
+@pytest.mark.parametrize("ea,eb", [(-60, -66), (-108, -18), (-1, -125), (40, 50), (99, 0), (-100, 200 - 100)])
+@pytest.mark.parametrize("m,n,k", [(5, 40, 1040), (300, 264, 512)])
+def test_scales_whose_product_is_normal(ea, eb, m, n, k):
+    """From 2^-126 to where the result leaves fp32."""
+    g = gen(20, m, n)
+    a, _ = R.operand(g, m, k, 1)
+    b, _ = R.operand(g, n, k, 128)
+    sa, sb = powers(m, k, ea, 2), powers(R.blocks(n), k, eb, 1)
+    c = run_matmul(a, sa, b, sb, F32)
+    ref, size = R.matmul(a, sa, b, sb, None, False)
+    assert torch.isfinite(c).all() and c.abs().max() > 0
+    assert ((c.double() - ref).abs() <= R.matmul_bound(ref, size, k, torch.float32)).all()
+
+
+def test_scales_whose_product_is_the_largest():
+    """One product of ones, times 2^127."""
+    a = torch.zeros((3, 256), device="cuda")
+    b = torch.zeros((16, 256), device="cuda")
+    a[0, 3] = b[2, 3] = 1.0
+    c = run_matmul(a.to(torch.float8_e4m3fn), torch.full((3, 2), 2.0 ** 100, device="cuda"), b.to(torch.float8_e4m3fn), torch.full((1, 2), 2.0 ** 27, device="cuda"), F32)
+    assert c[0, 2] == 2.0 ** 127 and c.count_nonzero() == 1
+
+
+@pytest.mark.parametrize("ea,eb", [(-70, -70), (-108, -30), (-100, -60)])
+def test_scales_whose_product_is_below_normal(ea, eb):
+    """The product of scales is off by 2^-150 at most, a block's sum is below 448^2 * 128 < 2^24.7, and adding rounds once a block."""
+    g = gen(21, ea)
+    m, n, k = 70, 130, 1024
+    a, _ = R.operand(g, m, k, 1)
+    b, _ = R.operand(g, n, k, 128)
+    sa, sb = powers(m, k, ea, 2) * 1.3, powers(R.blocks(n), k, eb, 1) * 1.7
+    c = run_matmul(a, sa, b, sb, F32)
+    ref, size = R.matmul(a, sa, b, sb, None, False)
+    assert ((c.double() - ref).abs() <= R.matmul_bound(ref, size, k, torch.float32) + R.blocks(k) * 2.0 ** -125).all()
+
+
+def test_scales_whose_product_is_beyond_fp32():
+    a = torch.full((2, 128), 2.0, device="cuda")
+    a[1] = 0
+    b = torch.full((16, 128), 1.0, device="cuda").to(torch.float8_e4m3fn)
+    c = run_matmul(a.to(torch.float8_e4m3fn), torch.full((2, 1), 2.0 ** 100, device="cuda"), b, torch.full((1, 1), 2.0 ** 28, device="cuda"), F32)
+    assert (c[0] == float("inf")).all() and torch.isnan(c[1]).all()
