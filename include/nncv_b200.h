@@ -71,7 +71,7 @@ enum {
   NNCV_B200_ENOMEM = 7
 };
 
-enum { NNCV_B200_F32 = 0, NNCV_B200_F16 = 1, NNCV_B200_BF16 = 2, NNCV_B200_E4M3 = 3 /* operands of nncv_b200_matmul_e4m3 only */ };
+enum { NNCV_B200_F32 = 0, NNCV_B200_F16 = 1, NNCV_B200_BF16 = 2, NNCV_B200_E4M3 = 3 /* out_dtype of nncv_b200_rmsnorm and _gated_activation only */ };
 
 typedef struct {
   int compute_dtype; /* NNCV_B200_F32 (fp32 accuracy: three bf16 planes per operand, tcgen05; activations take 6 bytes an

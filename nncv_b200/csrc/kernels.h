@@ -320,7 +320,6 @@ struct GatedArgs {
   DType dtype = kF16;
   bool to_e4m3 = false;
   int M = 0, K = 0, act = 0;
-  int sm_count = 0;
 };
 cudaError_t launch_gated_activation(const GatedArgs& a, cudaStream_t st);
 // One scale for each 128 x 128 block.

@@ -3148,7 +3148,7 @@ int nncv_b200_gated_activation(const void* gate, const void* up, long long ld, v
   if ((rc = device_init())) return rc;
   GatedArgs a;
   a.gate = gate; a.up = up; a.ld = ld; a.out = out; a.scale = scale; a.dtype = (DType)dtype; a.to_e4m3 = out_dtype == NNCV_B200_E4M3;
-  a.M = M; a.K = K; a.act = act; a.sm_count = g_dev.sm_count;
+  a.M = M; a.K = K; a.act = act;
   LAUNCH(launch_gated_activation(a, (cudaStream_t)stream));
   return ok();
 }
@@ -3171,7 +3171,7 @@ int nncv_b200_quantize_e4m3(const void* x, long long ldx, int dtype, void* q, fl
     return ok();
   }
   GatedArgs a;
-  a.gate = x; a.ld = ldx; a.out = q; a.scale = scale; a.dtype = (DType)dtype; a.to_e4m3 = true; a.M = M; a.K = K; a.sm_count = g_dev.sm_count;
+  a.gate = x; a.ld = ldx; a.out = q; a.scale = scale; a.dtype = (DType)dtype; a.to_e4m3 = true; a.M = M; a.K = K;
   LAUNCH(launch_gated_activation(a, (cudaStream_t)stream));
   return ok();
 }
