@@ -17,7 +17,7 @@
 // multiply-adds and 180 of tensor-memory loads a block, and the two do not overlap; sixteen epilogue warps instead of eight were 7 %
 // slower, one release of both parts 2 %, one wait a part 3 %, halves of tiles in the last round no faster.
 // Middle sizes: what an SM takes in from L2, about 56 bytes a clock (a block of 128 x 128 is 32 KB: 600 clocks where its MMAs take 256).
-// Few rows: reading B (4.4 TB/s of 6.5 at 16 x 8192 x 8192), and for one small layer what is fixed: of the 6.4 us of 1 x 4096 x 4096
+// Few rows: reading B (4.4 TB/s of 6.5 at 16 x 8192 x 8192), and for one small layer what is fixed: of the 6.4 us of 1 x 4096 x 4096 (7.6 with B from memory)
 // 1.9 pass until the first block is here, 2 while B comes, 1.9 while the CTAs of a cluster meet and add up.
 #include <cuda.h>
 #include <cudaTypedefs.h>

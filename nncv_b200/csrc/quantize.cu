@@ -5,10 +5,12 @@
 // The least scale keeps 1 / s finite for a block of zeros.  What is not finite becomes NaN -- e4m3 has no infinity -- and leaves
 // the other values of its block as they are.
 //
-// All of it is bound by HBM.  Eight threads hold the 128 columns of a block: each has 16 of them, in two pieces of eight that lie 64
-// columns apart, so that what the eight load and store at once lies in a row.  (Eight values a thread, a 64-bit division for each block
-// and a test for infinities for each value took twice the time.)  Of the 6.5 TB/s of a copy: norm 4096 x 4096 bf16 with residual to e4m3 5.9
-// (19.8 us), gated SiLU 2048 x 8192 bf16 to e4m3 6.1 (13.7 us), 8192 x 2048 bf16 to e4m3 5.6 (9.0 us), 4096 x 4096 fp32 in blocks 5.9 (14.3 us).
+// Bound by HBM where rows are whole blocks on 16-byte boundaries.  Eight threads hold the 128 columns of a block: each has 16 of them, in two
+// pieces of eight that lie 64 columns apart, so that what the eight load and store at once lies in a row.  (Eight values a thread, a 64-bit division
+// for each block and a test for infinities for each value took twice the time.)  Of the 6.5 TB/s of a copy: norm 4096 x 4096 bf16 with residual to
+// e4m3 5.9 (20.0 us), gated SiLU 2048 x 8192 bf16 to e4m3 5.9 (14.3 us), 8192 x 2048 bf16 to e4m3 5.4 (9.4 us), 4096 x 4096 fp32 in blocks 5.8
+// (14.4 us).  Further from it: norms of few columns (65536 x 128 bf16 23.6 us where the bytes take 3.9), rows off those boundaries (gated 2048 x
+// 8191 40 us), fp32 norms wider than 6144 (1024 x 16384 48 us, the bytes 33.5).
 #include <type_traits>
 
 #include "activation.cuh"
@@ -196,29 +198,29 @@ __device__ __forceinline__ float silu16(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
   return x * reciprocal(1.0f + e);
 }
-// SiLU and sigmoid have far gates: beyond kFar, 1 + exp(-|x|) is 1, and below -kFar x / (1 + exp(-x)) is x exp(x).  exp(-x) passes fp32's range from
-// -88.7 on, and the hardware's reciprocal is 0 from -87.3 on, where the result is no zero yet and a large `up` makes an ordinary value of it.
-constexpr float kFar = 80.0f;
+// SiLU and sigmoid of far gates, below kFar, are x exp(x) and exp(x): there 1 + exp(-x) is exp(-x), which passes fp32's range from -88.7 on, and the
+// hardware's reciprocal of it is 0 from -87.3 on, where the result is no zero yet and a large `up` makes an ordinary value of it.
+constexpr float kFar = -87.0f;
 template <typename T> __device__ __forceinline__ bool any_far(const Raw<T>& r) {   // NaN is passed over
   const T* e = reinterpret_cast<const T*>(r.p);
   if constexpr (sizeof(T) == 4) {
-    float a = fabsf(e[0]);
+    float a = e[0];
 #pragma unroll
-    for (int i = 1; i < kV; ++i) a = fmaxf(a, fabsf(e[i]));
-    return a > kFar;
+    for (int i = 1; i < kV; ++i) a = fminf(a, e[i]);
+    return a < kFar;
   } else {
     using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
     const T2* p = reinterpret_cast<const T2*>(e);
-    T2 a = __habs2(p[0]);
+    T2 a = p[0];
 #pragma unroll
-    for (int i = 1; i < kV / 2; ++i) a = __hmax2(a, __habs2(p[i]));
-    return fmaxf(ef<T>(a.x), ef<T>(a.y)) > kFar;
+    for (int i = 1; i < kV / 2; ++i) a = __hmin2(a, p[i]);
+    return fminf(ef<T>(a.x), ef<T>(a.y)) < kFar;
   }
 }
 template <bool SILU>
 __device__ __forceinline__ float far_gate(float x) {
   const float h = expf(0.5f * x);
-  return x > 0.0f ? (SILU ? x : 1.0f) : (SILU ? x * h : h) * h;
+  return (SILU ? x * h : h) * h;
 }
 template <typename T, int ACT>
 __device__ __forceinline__ float near_gate(float x, int act) {
@@ -259,8 +261,7 @@ __device__ __forceinline__ void load_weight(const float* weight, int col0, int t
 
 // Rows of up to kAheadK: a CTA takes one row after the other, which stays in registers between the sum of squares and the result, so
 // that every tensor is read once; the next row is on its way while this one is worked on, and the weights stay in registers.
-// (With a CTA a row, loads were under way only in the first half of its life: 4096 x 4096 bf16 with residual to e4m3 23.5 us, now 19.8:
-// 5.9 TB/s.)
+// (With a CTA a row, loads were under way only in the first half of its life: 4096 x 4096 bf16 with residual to e4m3 23.5 us, so 20.0.)
 constexpr int kAheadK = 16384;
 template <typename T, bool VEC, bool Q, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 2 : 1)
@@ -340,7 +341,7 @@ rmsnorm_long_kernel(const T* x, long long ldx, const T* residual, const float* w
 
 // ---------------------------------------------------------------- (gated) activation -------
 // What a warp does whose blocks have a far gate, value by value through local memory: unrolled it took 20 registers of the kernel below, which lost a
-// third of its warps.
+// third of its warps.  (2048 x 8192 bf16 to e4m3 with a far gate in every block 61 us, in one of 55 21, in none 14.3.)
 template <typename T, bool Q, int ACT>
 __device__ __forceinline__ void gated_far(const T* gate, const T* up, void* out, float* scale, int col0, int t, int K, int act) {
   float z[kV];
@@ -348,7 +349,7 @@ __device__ __forceinline__ void gated_far(const T* gate, const T* up, void* out,
   for (int e = 0; e < kV; ++e) {
     const int col = col0 + piece_col(e / kPiece, t) + e % kPiece;
     const float x = col < K ? ef<T>(gate[col]) : 0.0f;
-    float y = fabsf(x) > kFar ? (act == kActSilu ? far_gate<true>(x) : far_gate<false>(x)) : near_gate<T, ACT>(x, act);
+    float y = x < kFar ? (act == kActSilu ? far_gate<true>(x) : far_gate<false>(x)) : near_gate<T, ACT>(x, act);
     if (up) y *= col < K ? ef<T>(up[col]) : 0.0f;
     z[e] = col < K ? y : 0.0f;
   }
@@ -359,7 +360,7 @@ __device__ __forceinline__ void gated_far(const T* gate, const T* up, void* out,
   else store_row<T, false>(static_cast<T*>(out), col0, t, K, v);
 }
 // The same as a call.  The kernel is faster around one but from 16 bits to e4m3 (2048 x 8192, call and body in place: sigmoid fp32 30.5 and 37.5 us,
-// bf16 15.9 and 20.7, to e4m3 23.4 and 20.6).
+// bf16 15.9 and 20.7, to e4m3 23.4 and 20.4).
 template <typename T, bool Q, int ACT>
 __device__ __noinline__ void gated_far_call(const T* gate, const T* up, void* out, float* scale, int col0, int t, int K, int act) {
   gated_far<T, Q, ACT>(gate, up, out, scale, col0, t, K, act);
@@ -475,7 +476,7 @@ cudaError_t rmsnorm_as(const RmsNormArgs& a, cudaStream_t st) {
     return launch_pdl(rmsnorm_long_kernel<T, VEC, Q>, dim3((unsigned)a.M), dim3(kLongThreads), 0, st, static_cast<const T*>(a.x), a.ldx,
                       static_cast<const T*>(a.residual), a.weight, a.eps, static_cast<T*>(a.sum), a.out, a.scale, a.K);
   const int threads = ((a.K + kGroup - 1) / kGroup * kLanes + 31) / 32 * 32;
-  // as many CTAs as find room at once: 768 threads an SM with 80 registers each (4096 x 4096: 512 23.9 us, 768 19.8, 1280 21.2), 1024 with 64
+  // as many CTAs as find room at once: 768 threads an SM with 80 registers each (4096 x 4096: 512 23.9 us, 768 19.8, 1280 21.2 before the present quotients), 1024 with 64
   auto kern = threads <= 384 ? rmsnorm_kernel<T, VEC, Q, 384> : threads <= 512 ? rmsnorm_kernel<T, VEC, Q, 512> : rmsnorm_kernel<T, VEC, Q, 1024>;
   const long long grid = (long long)(a.sm_count > 0 ? a.sm_count : 148) * (threads <= 384 ? 768 / threads : 1024 / threads);
   return launch_pdl(kern, dim3((unsigned)(grid < a.M ? grid : a.M)), dim3(threads), 0, st, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.residual),
