@@ -140,8 +140,8 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 // Minus y / s for two values of a block.  The product with the approximate 1 / s is at most 2.5 steps of fp32 off; its remainder, by a fused
 // multiply-add, times 1 / s corrects it to 2^-21 of a step before the last rounding (after P. Markstein, Computation of elementary functions
 // on the IBM RISC System/6000, 1990).  So a quotient half way between two e4m3 values comes out as that and goes to the even one, where the
-// product alone sent some to the other.  The sign is turned twice, so that a zero keeps its own.  8192 x 2048 bf16
-// in rows takes 9.4 us, with the product alone 9.1; gated 2048 x 8192 13.9 for 13.7; 4096 x 4096 bf16 in blocks 12.3 for 11.6.
+// product alone sent some to the other.  The sign is turned twice, so that a zero keeps its own.  8192 x 2048 bf16 in rows takes 9.4 us, with the
+// product alone 9.1; 4096 x 4096 bf16 in blocks 12.3 for 11.6.
 struct Divisor {
   unsigned long long s, minus_inv;
   __device__ __forceinline__ explicit Divisor(float by) : s(epi::pk(by, by)) {
@@ -392,11 +392,11 @@ gated_kernel(const T* gate, const T* up, long long ld, void* out, float* scale, 
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
     if ((ACT == kActSilu || (ACT < 0 && (act == kActSilu || act == kActSigmoid))) && __any_sync(0xffffffffu, any_far<T>(g[i]))) {
-      const T *far_gate = gate + row[i] * ld, *far_up = UP ? up + row[i] * ld : nullptr;
-      void* to = static_cast<uint8_t*>(out) + row[i] * K * (Q ? 1 : (long long)sizeof(T));
+      const T *gate_row = gate + row[i] * ld, *up_row = UP ? up + row[i] * ld : nullptr;
+      void* out_row = static_cast<uint8_t*>(out) + row[i] * K * (Q ? 1 : (long long)sizeof(T));
       float* to_scale = Q ? scale + row[i] * kb.d + col0[i] / kGroup : nullptr;
-      if (!VEC || !Q || sizeof(T) == 4) gated_far_call<T, Q, ACT>(far_gate, far_up, to, to_scale, col0[i], t, K, act);
-      else gated_far<T, Q, ACT>(far_gate, far_up, to, to_scale, col0[i], t, K, act);
+      if (!VEC || !Q || sizeof(T) == 4) gated_far_call<T, Q, ACT>(gate_row, up_row, out_row, to_scale, col0[i], t, K, act);
+      else gated_far<T, Q, ACT>(gate_row, up_row, out_row, to_scale, col0[i], t, K, act);
       continue;
     }
     float v[kV];
@@ -476,7 +476,8 @@ cudaError_t rmsnorm_as(const RmsNormArgs& a, cudaStream_t st) {
     return launch_pdl(rmsnorm_long_kernel<T, VEC, Q>, dim3((unsigned)a.M), dim3(kLongThreads), 0, st, static_cast<const T*>(a.x), a.ldx,
                       static_cast<const T*>(a.residual), a.weight, a.eps, static_cast<T*>(a.sum), a.out, a.scale, a.K);
   const int threads = ((a.K + kGroup - 1) / kGroup * kLanes + 31) / 32 * 32;
-  // as many CTAs as find room at once: 768 threads an SM with 80 registers each (4096 x 4096: 512 23.9 us, 768 19.8, 1280 21.2 before the present quotients), 1024 with 64
+  // as many CTAs as find room at once: 768 threads an SM with 80 registers each (4096 x 4096: 512 23.9 us, 768 19.8, 1280 21.2, measured without
+  // the quotients' correction), 1024 with 64
   auto kern = threads <= 384 ? rmsnorm_kernel<T, VEC, Q, 384> : threads <= 512 ? rmsnorm_kernel<T, VEC, Q, 512> : rmsnorm_kernel<T, VEC, Q, 1024>;
   const long long grid = (long long)(a.sm_count > 0 ? a.sm_count : 148) * (threads <= 384 ? 768 / threads : 1024 / threads);
   return launch_pdl(kern, dim3((unsigned)(grid < a.M ? grid : a.M)), dim3(threads), 0, st, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.residual),
